@@ -1,8 +1,9 @@
 """Builds libcausal_conv1d_b200.so (the C-ABI library of include/causal_conv1d_b200.h) for
 sm_100a with nvcc, in-tree: objects under _build/, the library inside the Python package; then the
 package's CPython binding of the hot entry points (csrc/cc1d_pyfast.c -> _cc1d_fast*.so) and its
-torch-side forward/backward launchers (csrc/cc1d_torch_ext.cpp -> _cc1d_torch*.so, host C++ against
-torch's headers), both linked against that library.
+torch-side launchers (csrc/cc1d_torch_*.cpp -> _cc1d_torch*.so, host C++ against torch's headers),
+both linked against that library. An object is compiled again when one of the headers it includes
+is newer (nvcc's dependency list beside it).
 
     python causal-conv1d-triton_b200/build.py [--force] [--verbose]
 """
@@ -25,7 +26,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "causal_conv1d_b200", "libcausal_conv1d_b200.so")
 FAST_SRC = os.path.join(CSRC, "cc1d_pyfast.c")
 FAST = os.path.join(HERE, "causal_conv1d_b200", "_cc1d_fast" + sysconfig.get_config_var("EXT_SUFFIX"))
-TORCH_SRC = os.path.join(CSRC, "cc1d_torch_ext.cpp")
+TORCH_SRCS = [os.path.join(CSRC, f) for f in ("cc1d_torch_ext.cpp", "cc1d_torch_ssm.cpp")]
 TORCH_EXT = os.path.join(HERE, "causal_conv1d_b200", "_cc1d_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -51,6 +52,18 @@ def _headers():
     return hs + [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE) if f.endswith(".h")]
 
 
+def _deps(obj, src):
+    """What `obj` was compiled from: the files of this tree in its dependency list, or every header
+    before there is one."""
+    try:
+        with open(obj[:-2] + ".d") as f:
+            names = f.read().replace("\\\n", " ").split(":", 1)[1].split()
+    except (OSError, IndexError):
+        return [src] + _headers()
+    deps = [n for n in names if os.path.abspath(n).startswith(ROOT)]
+    return [src] + [n if os.path.exists(n) else src for n in deps]
+
+
 def _stale(target, deps) -> bool:
     if not os.path.exists(target):
         return True
@@ -66,15 +79,14 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     them with a separate `lib_path` and `build_dir`."""
     os.makedirs(build_dir, exist_ok=True)
     nvcc = _nvcc()
-    headers = _headers()
     srcs = sources()
     objs = [os.path.join(build_dir, os.path.basename(s)[:-3] + ".o") for s in srcs]
     dflags = [f"-D{d}" for d in defines]
-    todo = [(s, o) for s, o in zip(srcs, objs) if force or ptxas_verbose or _stale(o, [s] + headers)]
+    todo = [(s, o) for s, o in zip(srcs, objs) if force or ptxas_verbose or _stale(o, _deps(o, s))]
 
     def compile_one(so):
         s, o = so
-        cmd = [nvcc] + NVCC_FLAGS + dflags + (["-Xptxas", "-v"] if ptxas_verbose else []) + ["-c", s, "-o", o]
+        cmd = [nvcc] + NVCC_FLAGS + dflags + (["-Xptxas", "-v"] if ptxas_verbose else []) + ["-MMD", "-MF", o[:-2] + ".d", "-c", s, "-o", o]
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
@@ -121,7 +133,9 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     """Compiles the torch-side launchers (host C++, torch's headers and libraries) against the built
     library."""
     header = os.path.join(INCLUDE, "causal_conv1d_b200.h")
-    if not (force or _stale(TORCH_EXT, [TORCH_SRC, header, LIB])):
+    objs = [os.path.join(BUILD, os.path.basename(s)[:-4] + ".o") for s in TORCH_SRCS]
+    todo = [(s, o) for s, o in zip(TORCH_SRCS, objs) if force or _stale(o, [s, header])]
+    if not (todo or _stale(TORCH_EXT, objs + [LIB])):
         return TORCH_EXT
     import torch
     import torch.utils.cpp_extension as ce
@@ -129,19 +143,24 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     cxx = shutil.which("g++") or "c++"
     torch_lib = ce.library_paths()[0]
     cuda_inc = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-           "-DTORCH_EXTENSION_NAME=_cc1d_torch", "-DTORCH_API_INCLUDE_EXTENSION_H"]
+    flags = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+             "-DTORCH_EXTENSION_NAME=_cc1d_torch", "-DTORCH_API_INCLUDE_EXTENSION_H"]
     for inc in ce.include_paths() + [cuda_inc, sysconfig.get_paths()["include"], INCLUDE]:
-        cmd += ["-I", inc]
-    cmd += [TORCH_SRC, "-L", os.path.dirname(LIB), "-lcausal_conv1d_b200", "-L", torch_lib, "-lc10", "-lc10_cuda",
-            "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}",
-            "-o", TORCH_EXT]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"torch launcher build failed:\n{r.stdout}\n{r.stderr}")
+        flags += ["-I", inc]
+    link = [cxx, "-shared"] + objs + ["-L", os.path.dirname(LIB), "-lcausal_conv1d_b200", "-L", torch_lib, "-lc10",
+                                      "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN",
+                                      f"-Wl,-rpath,{torch_lib}", "-o", TORCH_EXT]
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"torch launcher build failed:\n{r.stdout}\n{r.stderr}")
+
+    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+        list(ex.map(lambda so: run([cxx] + flags + ["-c", so[0], "-o", so[1]]), todo))
+    run(link)
     return TORCH_EXT
 
 

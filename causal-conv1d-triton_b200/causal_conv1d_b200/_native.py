@@ -3,9 +3,10 @@
 `lib` binds every entry point with ctypes. `fast` is the package's CPython binding of the hot
 launch entry points (cc1d_fwd, cc1d_bwd_workspace_bytes, cc1d_bwd, cc1d_update; built from
 csrc/cc1d_pyfast.c), which parses arguments in a fraction of ctypes' per-call time. `tex` holds
-the forward and backward launchers written in C++ against torch (csrc/cc1d_torch_ext.cpp): they
-allocate the outputs and the workspace with torch's allocator and call cc1d_fwd / cc1d_bwd, which
-keeps the per-call host time of the autograd path low. All three reach the same loaded library and
+the forward and backward launchers written in C++ against torch (csrc/cc1d_torch_ext.cpp, and
+csrc/cc1d_torch_ssm.cpp for the state-space operators): they allocate the outputs and the workspace
+with torch's allocator and call the C entry points, which keeps the per-call host time of the
+autograd path low. All three reach the same loaded library and
 are built in-tree by causal-conv1d-triton_b200/build.py. Importing this module without them raises
 ImportError: there is no CPU or Python fallback for the kernels.
 """
@@ -40,8 +41,38 @@ class DoutPiece(ctypes.Structure):
                 ("stride_time", ctypes.c_int64), ("channels", ctypes.c_int64)]
 
 
+class Tokens(ctypes.Structure):
+    """cc1d_tokens: a (batch, seqlen, ...) operand and its strides in elements."""
+
+    _fields_ = [("ptr", ctypes.c_void_p), ("stride_batch", ctypes.c_int64), ("stride_time", ctypes.c_int64),
+                ("stride_group", ctypes.c_int64)]
+
+
+class Param(ctypes.Structure):
+    """cc1d_param: a contiguous operand and its element type code."""
+
+    _fields_ = [("ptr", ctypes.c_void_p), ("dtype", ctypes.c_int)]
+
+
+class SsmProblem(ctypes.Structure):
+    """cc1d_ssm_problem."""
+
+    _fields_ = [(n, Tokens) for n in ("x", "dt", "z", "B", "C")] + [
+        (n, Param) for n in ("A", "D", "dt_bias", "initial_states")] + [("seq_idx", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("batch", "seqlen", "dim", "dstate", "groups")] + [
+        ("x_dtype", ctypes.c_int), ("dt_softplus", ctypes.c_int)]
+
+
+class SsmGrads(ctypes.Structure):
+    """cc1d_ssm_grads."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dx", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias",
+                                               "dinitial_states")]
+
+
 # Every symbol the header declares, with its ctypes signature.
 _P, _I64, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+_PROBLEM = ctypes.POINTER(SsmProblem)
 SIGNATURES = {
     "cc1d_abi_version": ([], _I),
     "cc1d_fwd": ([_P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
@@ -59,6 +90,13 @@ SIGNATURES = {
                         _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _I, _I, _I,
                         _I, _P], _I),
     "cc1d_copy_channels": ([_P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I, _P], _I),
+    "cc1d_ssm_kept_bytes": ([_I64, _I64, _I64, _I64], _I64),
+    "cc1d_ssm_workspace_bytes": ([_I64, _I64, _I64, _I64, _I64, _I], _I64),
+    "cc1d_ssm_fwd": ([_PROBLEM, _P, _P, _P, _P, _I, _I64, _P, _I64, _P, _I64, _P], _I),
+    "cc1d_ssm_bwd": ([_PROBLEM, ctypes.POINTER(Tokens), _P, ctypes.POINTER(Param), ctypes.POINTER(SsmGrads), _P,
+                      _I64, _P], _I),
+    "cc1d_ssm_update": ([_PROBLEM, _P, _I, _I64, _P, _P, _P], _I),
+    "cc1d_slot_maps": ([_P, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P], _I),
     "cc1d_selftest_wait_timeout": ([_P], _I),
     "cc1d_status": ([ctypes.POINTER(ctypes.c_uint32), _I], _I),
     "cc1d_error_string": ([_I], ctypes.c_char_p),

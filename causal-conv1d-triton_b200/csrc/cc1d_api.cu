@@ -105,6 +105,20 @@ int occupancy(const KernelInfo& k, int max_smem, int dev, int* occ) {
   return CC1D_OK;
 }
 
+}  // namespace
+
+// For the entry points in other files.
+int record_cuda_error(cudaError_t e) { return cuda_fail(e); }
+int device_sms(int* sms) {
+  DeviceInfo di;
+  int dev = 0;
+  CC1D_TRY(device_info(&di, &dev));
+  *sms = di.sms;
+  return CC1D_OK;
+}
+
+namespace {
+
 int tensor_map_encoder(PFN_cuTensorMapEncodeTiled_v12000* fn) {
   std::lock_guard<std::mutex> lk(g_mu);
   if (g_encode == nullptr) {
@@ -588,7 +602,7 @@ const char* cc1d_error_string(int code) {
   switch (code) {
     case CC1D_OK: return "success";
     case CC1D_ERR_INVALID: return "invalid argument (size, stride, dtype code or missing pointer)";
-    case CC1D_ERR_UNSUPPORTED: return "unsupported width (the largest supported width is 256)";
+    case CC1D_ERR_UNSUPPORTED: return "unsupported size (the largest width is 256, the largest state 64 per channel)";
     case CC1D_ERR_WORKSPACE: return "workspace smaller than cc1d_bwd_workspace_bytes()";
     case CC1D_ERR_CUDA: return "CUDA call failed (see cc1d_last_cuda_error())";
     case CC1D_ERR_SCRATCH_LIMIT:

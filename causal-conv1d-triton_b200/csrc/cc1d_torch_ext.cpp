@@ -184,6 +184,8 @@ torch::autograd::variable_list conv_fn(const at::Tensor& x, const at::Tensor& we
 
 }  // namespace
 
+void bind_ssm(pybind11::module_& m);  // cc1d_torch_ssm.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "torch-side launchers of libcausal_conv1d_b200 (forward and backward)";
   m.def("fwd", &fwd, "(rc, out) = fwd(x, weight, bias, seq_idx, initial_states, final_states, silu)");
@@ -193,4 +195,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bwd", &bwd,
         "(rc, dx, dweight, dbias, dinit) = bwd(x, weight, bias, seq_idx, initial_states, dout, dfinal_states, "
         "need_dinit, silu, grad_f32, fuse_param_grads)");
+  bind_ssm(m);
 }

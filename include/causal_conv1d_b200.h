@@ -39,7 +39,7 @@ enum { CC1D_F32 = 0, CC1D_F16 = 1, CC1D_BF16 = 2 };
 enum {
   CC1D_OK = 0,
   CC1D_ERR_INVALID = 1,     /* bad size, stride, dtype code or missing required pointer */
-  CC1D_ERR_UNSUPPORTED = 2, /* width above the largest supported (256) */
+  CC1D_ERR_UNSUPPORTED = 2, /* width above the largest supported (256), or state above 64 */
   CC1D_ERR_WORKSPACE = 3,   /* workspace smaller than cc1d_bwd_workspace_bytes() */
   CC1D_ERR_CUDA = 4,        /* a CUDA runtime/driver call failed; see cc1d_last_cuda_error() */
   CC1D_ERR_SCRATCH_LIMIT = 5, /* cc1d_bwd_noalloc: problem needs more than its fixed scratch */
@@ -196,6 +196,111 @@ int cc1d_copy_channels(void* dst, int64_t dst_stride_batch, int64_t dst_stride_t
                        const void* src, int64_t src_stride_batch, int64_t src_stride_time,
                        int64_t batch, int64_t seqlen, int64_t channels, int elem_bytes,
                        void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * State-space operators: what a Mamba-style layer runs on the convolution's output. No counterpart
+ * in the reference, whose README names that layer as its caller. For each batch row, channel d and
+ * state n, with delta = softplus(dt + dt_bias) (or dt + dt_bias),
+ *
+ *   h[t] = exp(delta[t] A[d, n]) h[t-1] + delta[t] x[t] B[t, n]
+ *   out[t] = (sum_n C[t, n] h[t] + D[d] x[t]) silu(z[t])
+ *
+ * All arithmetic and h are fp32; x, dt, z, B, C, out and their gradients have one element type.
+ * --------------------------------------------------------------------------------------------- */
+
+/* Element (b, t, c) at ptr + b*stride_batch + t*stride_time + c elements; for B and C, state n of
+ * group g at ptr + b*stride_batch + t*stride_time + g*stride_group + n. */
+typedef struct cc1d_tokens {
+  const void* ptr;
+  int64_t stride_batch, stride_time, stride_group;
+} cc1d_tokens;
+
+/* A contiguous operand with its element type code; ptr NULL: absent. */
+typedef struct cc1d_param {
+  const void* ptr;
+  int dtype;
+} cc1d_param;
+
+typedef struct cc1d_ssm_problem {
+  cc1d_tokens x, dt;         /* (batch, seqlen, dim) */
+  cc1d_tokens z;             /* (batch, seqlen, dim); ptr NULL: no gate */
+  cc1d_tokens B, C;          /* (batch, seqlen, groups, dstate); channel d uses group d / (dim / groups) */
+  cc1d_param A, D, dt_bias;  /* (dim, dstate), (dim), (dim); D and dt_bias may be absent */
+  cc1d_param initial_states; /* (batch, dim, dstate): h before the first token; absent: zero */
+  const int32_t* seq_idx;    /* (batch, seqlen) or NULL: sequences packed in a row, as for cc1d_fwd: h starts from
+                                zero where the id changes, negative ids are padding whose outputs and gradients are 0 */
+  int64_t batch, seqlen, dim, dstate, groups; /* dim a multiple of groups; dstate 1..64 */
+  int x_dtype;               /* of x, dt, z, B, C and out */
+  int dt_softplus;           /* 0: delta = dt + dt_bias */
+} cc1d_ssm_problem;
+
+/* Bytes of the states that cc1d_ssm_fwd keeps for cc1d_ssm_bwd (h before every 16th token, fp32). */
+int64_t cc1d_ssm_kept_bytes(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate);
+
+/* Bytes of the workspace of cc1d_ssm_fwd (backward 0) or cc1d_ssm_bwd (1) on the current device; -1
+ * for invalid sizes. 0 for a forward that runs in one piece. */
+int64_t cc1d_ssm_workspace_bytes(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t groups, int backward);
+
+/*
+ * Forward over a sequence.
+ *   out           (batch, seqlen, dim) contiguous, type x_dtype
+ *   final_states  (batch, dim, dstate) fp32 or NULL: h after the last token
+ *   kept_states   cc1d_ssm_kept_bytes() bytes, or NULL when no backward follows
+ *   packed_state  (n_slots, dim, dstate) or NULL: with seq_idx, h after the last token of sequence id i of
+ *                 row b goes to slot packed_slots[b * packed_slots_n + i]; ids at or above packed_slots_n
+ *                 and slots outside [0, n_slots) are skipped
+ *   workspace     at least cc1d_ssm_workspace_bytes(..., 0) bytes
+ */
+int cc1d_ssm_fwd(const cc1d_ssm_problem* problem, void* out, float* final_states, float* kept_states,
+                 void* packed_state, int packed_state_dtype, int64_t n_slots, const int32_t* packed_slots,
+                 int64_t packed_slots_n, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients, contiguous: dx, ddt, dz (batch, seqlen, dim) and dB, dC (batch, seqlen, groups, dstate) of
+ * x_dtype; dA, dD, ddt_bias and dinitial_states of their operand's type. dz, dD and ddt_bias are
+ * required where their operand is given; dinitial_states may be NULL. */
+typedef struct cc1d_ssm_grads {
+  void *dx, *ddt, *dz, *dB, *dC, *dA, *dD, *ddt_bias, *dinitial_states;
+} cc1d_ssm_grads;
+
+/*
+ * Backward. kept_states as the forward of the same problem left it; dfinal_states (batch, dim, dstate)
+ * or NULL; workspace at least cc1d_ssm_workspace_bytes(..., 1) bytes. All sums over tokens, channels and
+ * CTAs are in a fixed order: the same inputs give the same bits.
+ */
+int cc1d_ssm_bwd(const cc1d_ssm_problem* problem, const cc1d_tokens* dout, const float* kept_states,
+                 const cc1d_param* dfinal_states, const cc1d_ssm_grads* grads, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
+/*
+ * New tokens (seqlen of them, usually one) against kept states.
+ *   state          (n_slots, dim, dstate) contiguous, updated in place
+ *   state_indices  (batch) slot of each row, or NULL for slot b; a slot outside [0, n_slots) skips the row
+ *                  (its output is left unwritten). Two rows of one call may not share a slot.
+ *   out            (batch, seqlen, dim) contiguous, type x_dtype
+ * seq_idx and initial_states of the problem are not used.
+ */
+int cc1d_ssm_update(const cc1d_ssm_problem* problem, void* state, int state_dtype, int64_t n_slots,
+                    const int32_t* state_indices, void* out, void* stream);
+
+/*
+ * The maps of a serving step from its requests' lengths, for a row of `seqlen` packed tokens:
+ *   lengths       (n) int32 new tokens of each request (a negative length counts as 0)
+ *   past_lengths  (n) int32 or NULL: tokens each request had before
+ *   slots         (n) int32 or NULL: state slot of each request, negative for none yet
+ *   free_slots    (n_free) int32: slots to hand out
+ *   cu_seqlens    (n + 1) out: request r is tokens [cu[r], cu[r+1]); edges past seqlen are cut to seqlen
+ *   seq_idx       (seqlen) out: each token's request, -1 past the last one
+ *   positions     (seqlen) out: its position in the request, counted from past_lengths; -1 past the last
+ *   tail_rows     (n, width - 1) out: the rows of each request's last width - 1 tokens, what a convolution
+ *                 of that width keeps; -1 for those before the request's first token
+ *   slots_out     (n) out, with slots: the slot of each request; a request with tokens and no slot takes the
+ *                 next of free_slots in request order (-1 once they are used up)
+ *   n_taken       (1) out: how many requests needed a new slot
+ */
+int cc1d_slot_maps(const int32_t* lengths, int64_t n, int64_t seqlen, int64_t width, const int32_t* past_lengths,
+                   const int32_t* slots, const int32_t* free_slots, int64_t n_free, int32_t* cu_seqlens,
+                   int32_t* seq_idx, int32_t* positions, int32_t* tail_rows, int32_t* slots_out, int32_t* n_taken,
+                   void* stream);
 
 /*
  * Reads the device status word of the current device after synchronising it, and clears it when

@@ -1,0 +1,498 @@
+"""The state-space scan, its single-token form and the slot maps on the GPU, against the 64-bit
+restatement (tests/_ssm_ref.py, which states how the tolerances follow from the arithmetic)."""
+
+import ctypes
+
+import pytest
+import torch
+
+import _ssm_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+GRADS = ("x", "dt", "A", "B", "C", "D", "z", "dt_bias", "initial_states")
+
+
+def to_dev(ops):
+    return {k: v.to(DEV) if torch.is_tensor(v) else v for k, v in ops.items()}
+
+
+def check_scan(ops, softplus=True, final=True, seed=7):
+    """Outputs, final states and every gradient of ssm_scan against the restatement."""
+    from causal_conv1d_b200 import ssm_scan
+
+    final = final and ops["seq_idx"] is None
+    g = torch.Generator().manual_seed(seed)
+    dout = torch.randn(ops["x"].shape, generator=g).to(ops["x"].dtype).to(DEV)
+    dfin = torch.randn(ops["x"].shape[0], ops["x"].shape[2], ops["A"].shape[1], generator=g).to(DEV)
+    mine, want = to_dev(ops), ref.wide(to_dev(ops))
+    names = [k for k in GRADS if ops[k] is not None]
+    for d in (mine, want):
+        for k in names:
+            d[k] = d[k].detach().clone().requires_grad_(True) if d[k].is_contiguous() else d[k].detach().requires_grad_(True)
+    res = ssm_scan(**mine, dt_softplus=softplus, return_final_states=final)
+    out, fin = res if final else (res, None)
+    wout, wh = ref.scan(**want, dt_softplus=softplus)
+    T = ops["x"].shape[1]
+    assert out.dtype == ops["x"].dtype
+    ref.assert_near(out, wout, T, "out")
+    got_out, got_in = [out], [dout]
+    exp_out, exp_in = [wout], [dout.double()]
+    if final:
+        assert fin.dtype == F32
+        ref.assert_near(fin, wh[:, -1], T, "final_states")
+        got_out, got_in = [out, fin], [dout, dfin]
+        exp_out, exp_in = [wout, wh[:, -1]], [dout.double(), dfin.double()]
+    got = torch.autograd.grad(got_out, [mine[k] for k in names], got_in)
+    exp = torch.autograd.grad(exp_out, [want[k] for k in names], exp_in)
+    for k, a, e in zip(names, got, exp):
+        assert a.dtype == ops[k].dtype, k
+        ref.assert_near(a, e, T, "d" + k)
+    with torch.no_grad():  # the form without a backward gives the same bits
+        again = ssm_scan(**{k: v.detach() if torch.is_tensor(v) else v for k, v in mine.items()}, dt_softplus=softplus,
+                         return_final_states=final)
+    assert torch.equal(again[0] if final else again, out.detach())
+    if final:
+        assert torch.equal(again[1], fin.detach())
+
+
+@pytest.mark.parametrize("batch, seqlen, dim, dstate, groups, dtype, kw", [
+    (1, 1, 1, 1, 0, F32, {}),
+    (2, 1, 64, 16, 0, BF16, dict(init=True)),
+    (1, 2, 5, 3, 1, F32, dict(D=False)),
+    (2, 15, 8, 4, 2, F16, dict(z=False)),
+    (1, 16, 128, 16, 0, BF16, {}),
+    (3, 17, 33, 16, 3, F32, dict(init=True, bias=False)),
+    (2, 31, 40, 12, 1, BF16, dict(D=False, z=False, bias=False)),
+    (1, 33, 130, 16, 0, F16, dict(init=True)),
+    (2, 70, 64, 17, 4, F32, dict(init=True)),
+    (1, 48, 72, 32, 0, BF16, {}),
+    (2, 37, 20, 33, 5, F32, {}),
+    (1, 65, 96, 64, 2, F16, dict(init=True)),
+    (1, 40, 257, 64, 0, F32, dict(z=False)),
+    (5, 64, 516, 16, 3, BF16, dict(init=True)),
+])
+def test_scan_and_gradients(batch, seqlen, dim, dstate, groups, dtype, kw):
+    check_scan(ref.case(seqlen * 31 + dim, batch, seqlen, dim, dstate, groups, dtype, **kw))
+
+
+@pytest.mark.parametrize("softplus", [False, True])
+def test_plain_steps(softplus):
+    """Without softplus the step is dt + dt_bias as given, negative ones among them."""
+    ops = ref.case(3, 2, 20, 24, 16)
+    if not softplus:
+        ops["dt"], ops["dt_bias"] = 0.02 * ops["dt"], 0.02 * ops["dt_bias"]
+    check_scan(ops, softplus=softplus)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim, dstate, groups", [(32, 16, 0), (40, 20, 2)])
+@pytest.mark.parametrize("init", [False, True])
+def test_packed(dtype, dim, dstate, groups, init):
+    """Sequences that start inside, at and just past the 16- and 32-token tiles, single tokens, padding
+    between and around them, a row that is padding alone."""
+    check_scan(ref.case(11, 4, 67, dim, dstate, groups, dtype, init=init, lengths=[
+        [67], [1, 15, 16, 1, -3, 31], [-2, 30, -1, 1, 33], [-67]]))
+
+
+def pieces(ops, backward):
+    from causal_conv1d_b200 import _native
+
+    b, t, d = ops["x"].shape
+    groups = ops["B"].shape[2] if ops["B"].ndim == 4 else 1
+    ws = _native.lib.cc1d_ssm_workspace_bytes(b, t, d, ops["A"].shape[1], groups, int(backward))
+    np = 4 * (4 if ops["A"].shape[1] <= 16 else 8 if ops["A"].shape[1] <= 32 else 16)
+    if not backward:
+        return max(1, ws // 4 // (2 * b * d * np))
+    blocks = groups * -(-(d // groups) // (512 * 4 // np))
+    rest = ws // 4 - b * t * blocks * 2 * np
+    one = b * (d * np + 2 * d)
+    return 1 if rest == one else (rest // (one + 2 * b * d * np))
+
+
+@pytest.mark.parametrize("kw", [dict(init=True), dict(lengths=[[300, 1, 255, -44, 424, -7, 469]])])
+@pytest.mark.parametrize("dim, dstate, dtype", [(24, 16, F32), (8, 40, F32), (64, 16, BF16)])
+def test_sequence_in_pieces(dim, dstate, dtype, kw):
+    """Few rows and channels: the sequence is cut, and states and gradients pass between pieces."""
+    ops = ref.case(5, 1, 1500, dim, dstate, 0, dtype, **kw)
+    assert pieces(ops, False) > 2 and pieces(ops, True) > 2
+    check_scan(ops)
+
+
+def test_gradients_match_differences():
+    """The derivative along a direction in every input, by central differences of the 64-bit form."""
+    from causal_conv1d_b200 import ssm_scan
+
+    ops = to_dev(ref.case(17, 2, 24, 24, 16, 2, init=True))
+    names = [k for k in GRADS if ops[k] is not None]
+    mine = {k: v.clone().requires_grad_(True) if k in names else v for k, v in ops.items()}
+    g = torch.Generator().manual_seed(1)
+    w = torch.randn(ops["x"].shape, generator=g).to(DEV)
+    grads = torch.autograd.grad(ssm_scan(**mine, dt_softplus=True), [mine[k] for k in names], w)
+    base = ref.wide(ops)
+    for k, d in zip(names, grads):
+        v = torch.randn(ops[k].shape, generator=g).to(DEV).double()
+
+        def f(e):
+            return (ref.scan(**{**base, k: base[k] + e * v}, dt_softplus=True)[0] * w.double()).sum()
+
+        # Central differences at 1e-5 in 64 bits: 1e-10 of cut-off and rounding; the rest is the gradient's own error.
+        want = (f(1e-5) - f(-1e-5)) / 2e-5
+        scale = (d.double() * v).abs().sum()
+        assert ((d.double() * v).sum() - want).abs() <= 1e-6 * 56 * scale, k
+
+
+def test_values_at_padding_do_not_matter():
+    """NaN and infinities in padded places, and in a sequence next to others, stay where they are."""
+    from causal_conv1d_b200 import ssm_scan
+
+    ops = to_dev(ref.case(23, 2, 50, 40, 16, lengths=[[10, -5, 35], [-20, 20, -10]]))
+    names = [k for k in GRADS if ops[k] is not None]
+    dout = torch.randn(2, 50, 40, device=DEV)
+
+    def run(o, d):
+        o = {k: v.clone().requires_grad_(True) if k in names else v for k, v in o.items()}
+        out = ssm_scan(**o, dt_softplus=True)
+        return (out, *torch.autograd.grad(out, [o[k] for k in names], d))
+
+    clean = run(ops, dout)
+    off = ops["seq_idx"] < 0
+    for bad in (float("nan"), float("inf"), torch.finfo(F32).min):
+        dirty = {k: v.clone() if torch.is_tensor(v) else v for k, v in ops.items()}
+        for k in ("x", "dt", "B", "C", "z"):
+            dirty[k][off] = bad
+        d = dout.clone()
+        d[off] = bad
+        for a, e in zip(run(dirty, d), clean):
+            assert torch.equal(a, e)
+    assert (clean[0][off] == 0).all() and (clean[1][off] == 0).all()
+
+    # An overflowing first sequence leaves the second one's outputs and token gradients alone.
+    dirty = {k: v.clone() if torch.is_tensor(v) else v for k, v in ops.items()}
+    dirty["x"][0, :10] = float("inf")
+    got = run(dirty, dout)
+    assert torch.equal(got[0][0, 10:], clean[0][0, 10:])
+    for k, a, e in zip(names, got[1:], clean[1:]):
+        if k in ("x", "dt", "B", "C", "z"):
+            assert torch.equal(a[0, 10:], e[0, 10:]), k
+
+
+def test_decay_extremes():
+    """Steps whose decay underflows to 0, steps of 0 (decay 1, no input), and a large softplus argument."""
+    ops = ref.case(29, 1, 20, 16, 16)
+    ops["dt_bias"] = None
+    ops["dt"] = torch.tensor([0.0, 1.0, 30.0, 200.0]).repeat(4)[None, None].expand(1, 20, 16).contiguous()
+    check_scan(ops, softplus=False)
+    ops["dt"] = torch.tensor([-80.0, -15.0, 21.0, 90.0]).repeat(4)[None, None].expand(1, 20, 16).contiguous()
+    check_scan(ops, softplus=True)
+
+
+def test_packed_states_go_to_slots():
+    from causal_conv1d_b200 import ssm_scan
+
+    ops = to_dev(ref.case(31, 2, 60, 24, 16, dtype=BF16, lengths=[[20, 1, -4, 35], [-10, 32, 18]]))
+    _, h = ref.scan(**ref.wide(ops), dt_softplus=True)
+    for dtype in (F32, BF16):
+        cache = torch.full((9, 24, 16), 7.0, device=DEV, dtype=dtype)
+        slots = torch.tensor([[4, 0, 8], [-1, 2, 5]], device=DEV)  # the second row has two sequences: 5 is not used
+        with torch.no_grad():
+            out = ssm_scan(**ops, dt_softplus=True, ssm_state=cache, ssm_state_indices=slots)
+            assert torch.equal(out, ssm_scan(**ops, dt_softplus=True))
+        for slot, (b, t) in {4: (0, 19), 0: (0, 20), 8: (0, 59), 2: (1, 59)}.items():
+            ref.assert_near(cache[slot], h[b, t], 60, f"slot {slot}")
+        for slot in (1, 3, 5, 6, 7):
+            assert (cache[slot] == 7).all()
+    # Ids without an entry and slots outside the buffer are skipped.
+    cache = torch.full((3, 24, 16), 7.0, device=DEV)
+    with torch.no_grad():
+        ssm_scan(**ops, dt_softplus=True, ssm_state=cache, ssm_state_indices=torch.tensor([[3], [1]], device=DEV))
+    assert (cache[0] == 7).all() and (cache[2] == 7).all()
+    ref.assert_near(cache[1], h[1, 41], 60)
+    with pytest.raises(AssertionError):
+        ops["x"].requires_grad_(True)
+        ssm_scan(**ops, ssm_state=cache, ssm_state_indices=slots)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_strides_and_alignment(dtype):
+    """Operands as slices of wider projections at odd offsets, transposed and expanded ones."""
+    from causal_conv1d_b200 import ssm_scan
+
+    base = to_dev(ref.case(37, 2, 33, 48, 16, dtype=dtype))
+    plain = ssm_scan(**base, dt_softplus=True)
+
+    def slice_of(t, offset, extra):
+        wide = torch.zeros(*t.shape[:-1], t.shape[-1] + extra, device=DEV, dtype=t.dtype)
+        wide[..., offset:offset + t.shape[-1]] = t
+        return wide[..., offset:offset + t.shape[-1]]
+
+    for offset in (1, 4, 8):
+        ops = {k: slice_of(v, offset, 24) if k in ("x", "dt", "B", "C", "z") else v for k, v in base.items()}
+        assert torch.equal(ssm_scan(**ops, dt_softplus=True), plain)
+        check_scan(ops)
+    ops = {k: v.transpose(0, 1).contiguous().transpose(0, 1) if k in ("x", "dt", "z") else v for k, v in base.items()}
+    ops["B"] = base["B"].transpose(1, 2).contiguous().transpose(1, 2)  # not contiguous along dstate
+    assert torch.equal(ssm_scan(**ops, dt_softplus=True), plain)
+    # B shared by the batch through a zero stride; a gradient without a channel stride of 1.
+    ops = {k: v.clone().requires_grad_(True) if k in ("x", "B") else v for k, v in base.items()}
+    one = ops["B"][:1]
+    out = ssm_scan(**{**ops, "B": one.expand(2, -1, -1)}, dt_softplus=True)
+    dout = torch.randn(2, 48, 33, device=DEV, dtype=dtype).transpose(1, 2)
+    (got,) = torch.autograd.grad(out, [ops["B"]], dout)
+    want = ref.wide({k: v.detach() if torch.is_tensor(v) else v for k, v in base.items()})
+    wb = want["B"][:1].clone().requires_grad_(True)
+    wout, _ = ref.scan(**{**want, "B": wb.expand(2, -1, -1)}, dt_softplus=True)
+    (exp,) = torch.autograd.grad(wout, [wb], dout.double())
+    # Two rounded rows added: twice the rounding of one.
+    off = (got[:1].double() - exp).abs()
+    assert (off <= 1e-6 * 65 * exp.abs().max() + 3 * ref.ROUND[dtype] * exp.abs().max()).all()
+    assert (got[1] == 0).all()
+
+
+def test_only_some_inputs_need_gradients():
+    from causal_conv1d_b200 import ssm_scan
+
+    ops = to_dev(ref.case(41, 2, 20, 24, 16, init=True))
+    full = {k: v.clone().requires_grad_(True) if k in GRADS else v for k, v in ops.items()}
+    w = torch.randn(2, 20, 24, device=DEV)
+    out, fin = ssm_scan(**full, dt_softplus=True, return_final_states=True)
+    everything = dict(zip(GRADS, torch.autograd.grad([out], [full[k] for k in GRADS], [w])))  # nothing comes back from fin
+    for k in GRADS:
+        some = dict(ops, **{k: ops[k].clone().requires_grad_(True)})
+        (g,) = torch.autograd.grad(ssm_scan(**some, dt_softplus=True), [some[k]], w)
+        assert torch.equal(g, everything[k]), k
+
+
+def test_parameter_types():
+    """A, D, dt_bias and the initial states in 16 bits and in 64."""
+    for dtype in (BF16, torch.float64):
+        ops = ref.case(43, 2, 18, 24, 16, init=True)
+        for k in ("A", "D", "dt_bias", "initial_states"):
+            ops[k] = ops[k].to(BF16).to(dtype)
+        if dtype == BF16:
+            check_scan(ops)
+        else:
+            from causal_conv1d_b200 import ssm_scan
+
+            o = to_dev(ops)
+            o["A"].requires_grad_(True)
+            out = ssm_scan(**o, dt_softplus=True)
+            (g,) = torch.autograd.grad(out.sum(), [o["A"]])
+            assert g.dtype == torch.float64
+            ref.assert_near(out, ref.scan(**ref.wide(to_dev(ops)), dt_softplus=True)[0], 18)
+
+
+def test_nothing_to_do():
+    from causal_conv1d_b200 import ssm_scan, ssm_update
+
+    for shape in ((2, 0, 8), (0, 5, 8), (2, 5, 0)):
+        ops = to_dev(ref.case(1, *shape, 4, init=True))
+        ops = {k: v.requires_grad_(True) if k in GRADS else v for k, v in ops.items()}
+        out, fin = ssm_scan(**ops, return_final_states=True)
+        assert out.shape == shape
+        if shape[1] == 0:
+            assert torch.equal(fin, ops["initial_states"])
+        grads = torch.autograd.grad([out, fin], [ops[k] for k in GRADS], [torch.ones_like(out), torch.ones_like(fin)])
+        for k, g in zip(GRADS, grads):
+            assert g.shape == ops[k].shape
+            assert (g == (1 if k == "initial_states" and shape[1] == 0 else 0)).all() or shape[0] == 0 or shape[2] == 0
+    ops = to_dev(ref.case(1, 2, 0, 8, 4))
+    state = torch.ones(2, 8, 4, device=DEV)
+    ops.pop("seq_idx"), ops.pop("initial_states")
+    assert ssm_update(ssm_state=state, **ops).shape == (2, 0, 8) and (state == 1).all()
+
+
+def test_same_bits_twice_and_on_another_stream():
+    from causal_conv1d_b200 import ssm_scan
+
+    ops = to_dev(ref.case(47, 2, 700, 96, 16, dtype=BF16))
+    names = [k for k in GRADS if ops[k] is not None]
+    dout = torch.randn(2, 700, 96, device=DEV).to(BF16)
+
+    def run():
+        o = {k: v.clone().requires_grad_(True) if k in names else v for k, v in ops.items()}
+        out = ssm_scan(**o, dt_softplus=True)
+        return (out, *torch.autograd.grad(out, [o[k] for k in names], dout))
+
+    first = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, e in zip(second, first):
+        assert torch.equal(a, e)
+
+
+def token_ops(ops, t):
+    return {k: v[:, t] if k in ("x", "dt", "B", "C", "z") and v is not None else v for k, v in ops.items()
+            if k not in ("seq_idx", "initial_states")}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("dim, dstate, groups", [(64, 16, 0), (33, 5, 3), (40, 64, 2), (24, 30, 1)])
+def test_decode_steps_equal_scan(dtype, dim, dstate, groups):
+    """Token by token, then several at a time: the scan's outputs and states, bit for bit."""
+    from causal_conv1d_b200 import ssm_scan, ssm_update
+
+    ops = to_dev(ref.case(53, 3, 12, dim, dstate, groups, dtype, init=True))
+    full, final = ssm_scan(**ops, dt_softplus=True, return_final_states=True)
+    state = ops["initial_states"].clone()
+    outs = [ssm_update(ssm_state=state, dt_softplus=True, **token_ops(ops, t)) for t in range(12)]
+    assert torch.equal(torch.stack(outs, 1), full) and torch.equal(state, final)
+    state = ops["initial_states"].clone()
+    outs = [ssm_update(ssm_state=state, dt_softplus=True, **token_ops(ops, slice(t, t + 5))) for t in (0, 5, 10)]
+    assert torch.equal(torch.cat(outs, 1), full) and torch.equal(state, final)
+
+
+@pytest.mark.parametrize("state_dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dstate", [16, 7])
+def test_update_slots(state_dtype, dstate):
+    from causal_conv1d_b200 import ssm_update
+
+    ops = to_dev(ref.case(59, 5, 1, 40, dstate, dtype=BF16, D=False))
+    state0 = torch.randn(8, 40, dstate, device=DEV).to(state_dtype)
+    slots = torch.tensor([6, -1, 0, 3, 9], device=DEV)  # one padded entry, one slot outside the buffer
+    state = state0.clone()
+    out = ssm_update(ssm_state=state, dt_softplus=True, ssm_state_indices=slots, **token_ops(ops, 0))
+    want = ref.wide(ops)
+    for i, s in ((0, 6), (2, 0), (3, 3)):
+        one = {k: v[i:i + 1] if k in ("x", "dt", "B", "C", "z") else v for k, v in want.items()}
+        one["initial_states"] = state0[s:s + 1].double()
+        wout, wh = ref.scan(**one, dt_softplus=True)
+        ref.assert_near(out[i:i + 1], wout[:, 0], 1, "out")
+        ref.assert_near(state[s], wh[0, 0], 1, "state")
+    for s in (1, 2, 4, 5, 7):
+        assert torch.equal(state[s], state0[s])
+
+
+def test_update_misaligned_state_and_offsets_past_32_bits():
+    from causal_conv1d_b200 import ssm_update
+
+    ops = token_ops(to_dev(ref.case(61, 2, 1, 2048, 16, dtype=BF16)), 0)
+    flat = torch.randn(2 * 2048 * 16 + 1, device=DEV)
+    a, b = flat[:-1].clone().view(2, 2048, 16), flat.clone()[1:].view(2, 2048, 16)
+    b.copy_(a)
+    assert b.data_ptr() % 16 != 0
+    oa, ob = (ssm_update(ssm_state=s, dt_softplus=True, **ops) for s in (a, b))
+    assert torch.equal(oa, ob) and torch.equal(a, b)
+    # 2.3e9 states of 16 bits: slots whose element offsets pass 2^31.
+    big = torch.zeros(70000, 2048, 16, device=DEV, dtype=BF16)
+    big[66000], big[69999] = flat[:-1].view(2, 2048, 16).to(BF16)
+    small = torch.stack([big[66000], big[69999]])
+    ob = ssm_update(ssm_state=big, dt_softplus=True, ssm_state_indices=torch.tensor([66000, 69999], device=DEV), **ops)
+    oa = ssm_update(ssm_state=small, dt_softplus=True, **ops)
+    assert torch.equal(oa, ob) and torch.equal(big[66000], small[0]) and torch.equal(big[69999], small[1])
+
+
+def test_scan_strides_past_32_bits():
+    """Tokens 2^30 elements apart: the last ones lie past 2^31."""
+    from causal_conv1d_b200 import ssm_scan
+
+    ops = to_dev(ref.case(67, 1, 3, 16, 4, dtype=BF16))
+    far = torch.zeros(2**31 + 64, device=DEV, dtype=BF16)
+    x = far.as_strided((1, 3, 16), (0, 2**30, 1))
+    x.copy_(ops["x"])
+    assert torch.equal(ssm_scan(**{**ops, "x": x}, dt_softplus=True), ssm_scan(**ops, dt_softplus=True))
+
+
+def test_update_in_a_graph():
+    from causal_conv1d_b200 import ssm_update
+
+    ops = token_ops(to_dev(ref.case(71, 4, 1, 64, 16, dtype=BF16)), 0)
+    state = torch.randn(4, 64, 16, device=DEV)
+    eager = state.clone()
+    want = [ssm_update(ssm_state=eager, dt_softplus=True, **ops) for _ in range(3)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    warm = state.clone()
+    with torch.cuda.stream(side):
+        ssm_update(ssm_state=warm, dt_softplus=True, **ops)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ssm_update(ssm_state=state, dt_softplus=True, **ops)
+    for w in want:
+        graph.replay()
+        assert torch.equal(out, w)
+    assert torch.equal(state, eager)
+
+
+def test_c_abi_through_ctypes():
+    """The header's structures as the package's ctypes binding lays them out."""
+    from causal_conv1d_b200 import _native as n
+    from causal_conv1d_b200 import ssm_scan
+
+    ops = to_dev(ref.case(73, 2, 40, 24, 16, 2, BF16, init=True))
+    want, final = ssm_scan(**ops, dt_softplus=True, return_final_states=True)
+    q = n.SsmProblem(batch=2, seqlen=40, dim=24, dstate=16, groups=2, x_dtype=2, dt_softplus=1)
+    for k in ("x", "dt", "z"):
+        setattr(q, k, n.Tokens(ops[k].data_ptr(), ops[k].stride(0), ops[k].stride(1), 0))
+    for k in ("B", "C"):
+        setattr(q, k, n.Tokens(ops[k].data_ptr(), *ops[k].stride()[:3]))
+    for k in ("A", "D", "dt_bias", "initial_states"):
+        setattr(q, k, n.Param(ops[k].data_ptr(), 0))
+    out, fin = torch.empty_like(want), torch.empty_like(final)
+    size = n.lib.cc1d_ssm_workspace_bytes(2, 40, 24, 16, 2, 0)
+    ws = torch.empty(max(1, size), device=DEV, dtype=torch.uint8)
+    stream = torch.cuda.current_stream().cuda_stream
+    n.check(n.lib.cc1d_ssm_fwd(ctypes.byref(q), out.data_ptr(), fin.data_ptr(), None, None, 0, 0, None, 0,
+                               ws.data_ptr(), size, stream), "cc1d_ssm_fwd")
+    assert torch.equal(out, want) and torch.equal(fin, final)
+
+
+def maps_by_hand(lengths, seqlen, width, slots, free, past):
+    cu, seq, pos, tail = [0], [-1] * seqlen, [-1] * seqlen, []
+    out, taken = [], 0
+    for r, k in enumerate(lengths):
+        k = max(k, 0)
+        start, end = cu[-1], min(seqlen, cu[-1] + k)
+        for i in range(start, end):
+            seq[i], pos[i] = r, i - start + (past[r] if past else 0)
+        tail.append([i if i >= start else -1 for i in range(end - width + 1, end)])
+        if slots is not None:
+            if slots[r] < 0 and k > 0:
+                out.append(free[taken] if taken < len(free) else -1)
+                taken += 1
+            else:
+                out.append(slots[r])
+        cu.append(end)
+    return cu, [seq], [pos], tail, out if slots is not None else None, [taken]
+
+
+@pytest.mark.parametrize("n, seqlen, width, most", [
+    (0, 10, 4, 1), (1, 1, 1, 1), (1, 0, 4, 5), (3, 17, 4, 9), (7, 1030, 8, 200), (40, 200, 2, 12), (257, 2048, 4, 9),
+    (4096, 9000, 4, 4), (4097, 9000, 3, 4), (5000, 4000, 2, 3),
+])
+@pytest.mark.parametrize("with_slots", [False, True])
+def test_slot_maps(n, seqlen, width, most, with_slots):
+    from causal_conv1d_b200 import slot_maps_from_lengths
+
+    g = torch.Generator().manual_seed(n + seqlen)
+    lengths = torch.randint(-1, most + 1, (n,), generator=g, dtype=torch.int32)  # zero and negative ones among them
+    slots = free = past = None
+    if with_slots:
+        slots = torch.where(torch.rand(n, generator=g) < 0.5, torch.arange(n), -1)
+        free = torch.arange(n, n + n // 3)  # fewer than are wanted
+        past = torch.randint(0, 99, (n,), generator=g)
+    got = slot_maps_from_lengths(lengths.to(DEV), seqlen, width, *(t.to(DEV) if t is not None else None for t in (slots, free, past)))
+    want = maps_by_hand(lengths.tolist(), seqlen, width, *(t.tolist() if t is not None else None for t in (slots, free, past)))
+    assert got._fields == ("cu_seqlens", "seq_idx", "positions", "tail_rows", "slots", "n_taken")
+    for name, a, e in zip(got._fields, got, want):
+        if e is None:
+            assert a is None
+        else:
+            assert a.dtype == torch.int32
+            assert a.tolist() == e, name
+
+
+def test_slot_maps_lengths_that_pass_32_bits():
+    from causal_conv1d_b200 import slot_maps_from_lengths
+
+    lengths = torch.tensor([5, 2**31 - 1, 2**31 - 1, 7], dtype=torch.int32, device=DEV)
+    got = slot_maps_from_lengths(lengths, 12, 2)
+    assert got.cu_seqlens.tolist() == [0, 5, 12, 12, 12]
+    assert got.seq_idx.tolist() == [[0] * 5 + [1] * 7]
+    with pytest.raises(AssertionError):
+        slot_maps_from_lengths(lengths, 12, slots=torch.zeros(4, dtype=torch.int32))  # not on the device
