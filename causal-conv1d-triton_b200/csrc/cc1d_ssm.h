@@ -42,8 +42,9 @@ struct SsmParams {
   int cache_dtype;
   const int32_t* cache_idx;    // (batch, cache_n) slot of each sequence id
   int64_t cache_n, cache_slots;  // ids per row that cache_idx covers; rows of cache (a slot outside is skipped)
-  // Sequences in pieces: what a piece starts from, and its decay (batch, segs, dim, 4 NL) each.
-  float *seg_state, *seg_decay;
+  // Sequences in pieces, (batch, segs, dim, 4 NL) each: the state (gradient) that a piece leaves when it
+  // receives none, its decay, and what it receives.
+  float *seg_out, *seg_decay, *seg_in;
   // Backward
   SsmTokens dout;
   SsmParam dfinal;             // (batch, dim, dstate) or null
@@ -67,6 +68,7 @@ struct SsmUpdateParams {
   void* out;               // (batch, seqlen, dim) contiguous
   int batch, seqlen, dim, dstate, group_dim;
   int softplus;
+  int blocks, state_vec;   // set by the launcher: CTAs over the channels; 4 states are one aligned vector
 };
 
 int record_cuda_error(cudaError_t e);  // sets cc1d_last_cuda_error(), returns CC1D_ERR_CUDA
@@ -74,8 +76,8 @@ int record_cuda_error(cudaError_t e);  // sets cc1d_last_cuda_error(), returns C
 // Lanes of a warp that share a channel, 4 states each: 4, 8 or 16. Fewer than 13 states run as 16
 // with zeros.
 inline int ssm_lanes(int dstate) { return dstate <= 16 ? 4 : dstate <= 32 ? 8 : 16; }
-inline int ssm_fwd_channels(int nl) { return 256 / nl; }  // channels of a forward CTA (256 threads)
-inline int ssm_bwd_channels(int nl) { return 512 / nl; }  // channels of a backward CTA (128 threads)
+// Channels of a CTA: 128 threads of two channels each, NL of them alike.
+inline int ssm_channels(int nl) { return 256 / nl; }
 
 enum SsmPass : int { kSsmForward = 0, kSsmPieceForward = 1, kSsmPieceBackward = 2 };
 

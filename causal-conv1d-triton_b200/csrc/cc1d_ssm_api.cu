@@ -31,11 +31,10 @@ struct Plan {
 // wait. `pass` is that pass's share of the main one, `launches` its fixed cost in tokens of one CTA,
 // `full` the time of an SM with two CTAs relative to one. The cheapest number of pieces is taken.
 Plan make_plan(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t groups, bool backward, int sms) {
-  const double pass = backward ? 0.4 : 0.9, launches = backward ? 40 : 150, full = backward ? 1.6 : 1.86;
+  const double pass = backward ? 0.25 : 0.75, launches = backward ? 35 : 100, full = backward ? 1.59 : 1.53;
   Plan r;
   r.nl = ssm_lanes(static_cast<int>(dstate));
-  const int ch = backward ? ssm_bwd_channels(r.nl) : ssm_fwd_channels(r.nl);
-  r.blocks = static_cast<int>(cdiv(dim / groups, ch));
+  r.blocks = static_cast<int>(cdiv(dim / groups, ssm_channels(r.nl)));
   r.segs = 1, r.seg_len = static_cast<int>(std::max<int64_t>(32, cdiv(seqlen, 32) * 32));
   const int64_t ctas = batch * groups * r.blocks, room = 2 * sms;
   const int64_t most = std::min<int64_t>(cdiv(2 * room, std::max<int64_t>(1, ctas)), cdiv(seqlen, 64));
@@ -65,7 +64,7 @@ int plan_for(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t
 }
 
 int64_t pieces_floats(const Plan& plan, int64_t batch, int64_t dim) {
-  return plan.segs > 1 ? 2 * batch * plan.segs * dim * 4 * plan.nl : 0;
+  return plan.segs > 1 ? 3 * batch * plan.segs * dim * 4 * plan.nl : 0;
 }
 
 int64_t bwd_floats(const Plan& plan, int64_t batch, int64_t seqlen, int64_t dim, int64_t groups) {
@@ -112,6 +111,10 @@ SsmParams common(const cc1d_ssm_problem& q, const Plan& plan) {
   p.group_dim = static_cast<int>(q.dim / q.groups), p.softplus = q.dt_softplus != 0;
   p.segs = plan.segs, p.seg_len = plan.seg_len, p.blocks = plan.blocks;
   return p;
+}
+
+void set_pieces(SsmParams& p, float* ws, int64_t floats) {
+  p.seg_out = ws, p.seg_decay = ws + floats / 3, p.seg_in = ws + 2 * (floats / 3);
 }
 
 int done(cudaError_t e) { return e == cudaSuccess ? CC1D_OK : record_cuda_error(e); }
@@ -161,7 +164,7 @@ int cc1d_ssm_fwd(const cc1d_ssm_problem* q, void* out, float* final_states, floa
   p.cache_slots = n_slots;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (plan.segs > 1) {
-    p.seg_state = static_cast<float*>(workspace), p.seg_decay = p.seg_state + need / 2;
+    set_pieces(p, static_cast<float*>(workspace), need);
     CC1D_TRY(done(launch_ssm_scan(p, kSsmPieceForward, q->x_dtype, s)));
     CC1D_TRY(done(launch_ssm_join(p, false, s)));
   }
@@ -191,16 +194,13 @@ int cc1d_ssm_bwd(const cc1d_ssm_problem* q, const cc1d_tokens* dout, const float
   p.dinit = grads->dinitial_states;
   const int64_t np = 4 * plan.nl, bs = q->batch * plan.segs, piece = pieces_floats(plan, q->batch, q->dim);
   float* ws = static_cast<float*>(workspace);
-  p.seg_state = ws, p.seg_decay = ws + piece / 2;
+  set_pieces(p, ws, piece);
   p.part_bc = ws + piece;
   p.part_a = p.part_bc + q->batch * q->seqlen * q->groups * plan.blocks * 2 * np;
   p.part_d = p.part_a + bs * q->dim * np;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (plan.segs > 1) {
-    SsmParams pieces = p;  // by the forward kernel's channel blocks
-    pieces.blocks = static_cast<int>(cdiv(p.group_dim, ssm_fwd_channels(plan.nl)));
-    if (q->batch * plan.segs * q->groups * pieces.blocks > kMaxInt) return CC1D_ERR_INVALID;
-    CC1D_TRY(done(launch_ssm_scan(pieces, kSsmPieceBackward, q->x_dtype, s)));
+    CC1D_TRY(done(launch_ssm_scan(p, kSsmPieceBackward, q->x_dtype, s)));
     CC1D_TRY(done(launch_ssm_join(p, true, s)));
   }
   return done(launch_ssm_bwd(p, q->x_dtype, s));

@@ -12,359 +12,400 @@
 namespace cc1d {
 namespace {
 
-constexpr int kThreads = 128, kWarps = 4;
-constexpr int kTokens = kSsmTile;  // tokens staged at a time: from one kept state to the next
-constexpr int kRun = 4;            // tokens whose decays and states a thread holds in registers
-
-template <typename T>
-__device__ __forceinline__ void copy_raw8(uint4* dst, const T* src, int n, bool vec, int stride) {
-  constexpr int Q = static_cast<int>(sizeof(T)) / 2;  // 16-byte pieces of 8 channels
-  if (vec && n == 8) {
-#pragma unroll
-    for (int i = 0; i < Q; ++i)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + i * stride)),
-                   "l"(reinterpret_cast<const uint4*>(src) + i)
-                   : "memory");
-  } else {
-    const Raw8<T> r = load8(src, n, false);
-#pragma unroll
-    for (int i = 0; i < Q; ++i) dst[i * stride] = make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void read_raw8(const uint4* src, int stride, float (&v)[8]) {
-  Raw8<T> r;
-#pragma unroll
-  for (int i = 0; i < Raw8<T>::NW / 4; ++i) {
-    const uint4 q = src[i * stride];
-    r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
-  }
-  unpack8(r, v);
-}
+constexpr int kThreads = 2 * kSsmHalf, kWarps = 4;  // warps of the walk
+constexpr int kTokens = kSsmTile;                  // tokens of a tile: from one kept state to the next
+constexpr int kRun = 4;                            // tokens whose decays and states a thread holds in registers
+constexpr int kBuffers = 2;                        // tiles handed over
+// Registers of a thread of each half after setmaxnreg; together twice what the launch gives each (128).
+constexpr int kWalkRegs = 152, kElementRegs = 104;
+static_assert(kWalkRegs + kElementRegs == 2 * 128, "the split draws on the registers of the launch");
 
 // Shared memory of one CTA.
 template <typename T, int NL>
 struct BwdSmem {
-  static constexpr int CH = 512 / NL, NP = 4 * NL, VR = CH / 8;
-  static constexpr int NV = (kTokens * VR + kThreads - 1) / kThreads;  // 8-channel vectors per thread of a tile
-  static constexpr int Q = static_cast<int>(sizeof(T)) / 2;
-  uint4 raw[2][4][NV][Q][kThreads];     // x, dt, z, dout as loaded; each thread reads only its own
-  float f[3][kTokens][CH];              // delta, delta x, dy; each token's then replaced by sum C h, sum g B, sum q A
-  float4 h[kTokens / kRun][4][kThreads];  // states before each run of kRun tokens, private to a thread
-  float4 bc[2][kTokens][NL];            // B, C
-  float dbc[kWarps][kTokens][2 * NP];   // each warp's dB and dC of the tile
-  float sk[2][CH];                      // D, dt_bias
-  float sum[16][kThreads];              // dD and ddt_bias of a thread's 8 channels
+  static constexpr int CH = 256 / NL, NP = 4 * NL, NQ = 2 * kTokens * NL / kSsmHalf;
+  // Handed over.
+  float4 du[kBuffers][kTokens][CH / 2];          // (delta, delta, delta x, delta x) of a channel pair
+  float f[kBuffers][3][kTokens][CH];             // dy, then sum C h; sum g B; sum q A
+  float4 bc[kBuffers][2][kTokens][NL];           // B, C
+  float dbc[kBuffers][kWarps][kTokens][2 * NP];  // each warp's dB and dC of the tile
+  uint32_t start[kBuffers];                      // SeqBits of the tile
+  // The walk's own, private to a thread: states before each run but the first, and before the tile.
+  float4 h[kTokens / kRun - 1][2][kSsmHalf];
+  float4 kept[2][2][kSsmHalf];
+  // The element-wise threads' own, as loaded: x, dt, z, dout; B and C; sequence ids.
+  uint4 raw[3][4][sizeof(T) / 2][kSsmHalf];
+  Raw4<T> raw_bc[2][NQ][kSsmHalf];
+  SeqIds ids[2][kWarps][kTokens];
+  float sk[2][CH];                               // D, dt_bias
 };
 
-// A lane holds 4 channels x 4 states, NL lanes a channel's states and 32 / NL lanes the warp's
-// channels: of each token's products, the sums over states (y, sum g B, sum q A) and over channels
-// (dB, dC) are first formed inside the thread, then across lanes by lane_sums, 12 values over NL
-// lanes and 8 over the rest, which leaves 16 shuffles per token for 16 (channel, state) pairs.
-// Bounded by the MUFU and FMA pipes: 1.75 exponentials and about 15 multiply-adds a pair.
+// The first four warps walk the tokens back, the other four do what is element-wise around them: dy,
+// (delta, delta x), B and C of the next tile, and from the sums of the last one dx, ddt, dz and the
+// CTA's dB and dC.
+//
+// In the walk a lane holds 2 channels x 4 states, NL lanes a channel's states and 32 / NL lanes the
+// warp's channels: of each token's products, the sums over states (y, sum g B, sum q A) and over
+// channels (dB, dC) are first formed inside the lane, then across lanes by lane_sums: 12 values of two
+// tokens over NL lanes, 8 of each token over the rest. A tile's states are first walked through,
+// keeping those before every 4th token, and each run of 4 tokens is then computed once more into
+// registers and walked back. All stores to shared memory of a run are at its end, so that nothing
+// keeps the loads of its next token from being issued early.
 // SEQ: packed rows (seq_idx), where a step may have to drop what came before it.
 template <typename T, int NL, bool SEQ>
-__global__ void __launch_bounds__(kThreads, 2) cc1d_ssm_bwd_kernel(const __grid_constant__ SsmParams p) {
+struct Bwd {
   using S = BwdSmem<T, NL>;
-  constexpr int CL = 32 / NL, CH = S::CH, NP = S::NP, VR = S::VR, NV = S::NV;
-  constexpr int QUADS = kTokens * NL, NQ = 2 * QUADS / kThreads;
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  S& s = *reinterpret_cast<S*>(smem_raw);
+  static constexpr int CL = 32 / NL, CH = S::CH, NP = S::NP, VR = CH / 8;
+  static constexpr int QUADS = kTokens * NL, NQ = S::NQ;
 
-  const SsmPlace w = ssm_place<CH>(p);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int nl = lane % NL, n0 = 4 * nl;
-  const int lc = warp * 4 * CL + 4 * (lane / NL);  // first of the thread's channels, within the block
-  const int64_t row_bs = static_cast<int64_t>(w.b) * p.segs + w.seg;
+  static __device__ __forceinline__ void elementwise(const SsmParams& p, const SsmPlace& w, S& s, int tiles) {
+    const int tid = threadIdx.x - kSsmHalf;
+    const int er = tid / VR, ec = (tid % VR) * 8, en = min(8, w.nc - ec);  // 8 channels of token er of a tile
+    const bool work = er < kTokens && en > 0;
+    const bool has_z = p.z.ptr != nullptr;
+    const T* const src[4] = {static_cast<const T*>(p.x.ptr) + w.b * p.x.sb + w.c0 + ec,
+                             static_cast<const T*>(p.dt.ptr) + w.b * p.dt.sb + w.c0 + ec,
+                             static_cast<const T*>(p.z.ptr) + w.b * p.z.sb + w.c0 + ec,
+                             static_cast<const T*>(p.dout.ptr) + w.b * p.dout.sb + w.c0 + ec};
+    const int64_t step[4] = {p.x.st, p.dt.st, p.z.st, p.dout.st};
+    const int vec[4] = {p.x.vec, p.dt.vec, p.z.vec, p.dout.vec};
+    const T* bp = static_cast<const T*>(p.Bm.ptr) + w.b * p.Bm.sb + w.g * p.Bm.sg;
+    const T* cp = static_cast<const T*>(p.Cm.ptr) + w.b * p.Cm.sb + w.g * p.Cm.sg;
+    SeqIds* const ids[2] = {&s.ids[0][tid >> 5][tid & 15], &s.ids[1][tid >> 5][tid & 15]};
 
-  for (int i = tid; i < CH; i += kThreads) {
-    const bool in = i < w.nc;
-    s.sk[0][i] = in && p.D.ptr != nullptr ? ld_any(p.D.ptr, w.c0 + i, p.D.dtype) : 0.0f;
-    s.sk[1][i] = in && p.dt_bias.ptr != nullptr ? ld_any(p.dt_bias.ptr, w.c0 + i, p.dt_bias.dtype) : 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) s.sum[i][tid] = 0.0f;
-
-  float2 A2[4][2], g[4][2], dA[4][2];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    float a[4], v[4];
-    const int ch = w.c0 + lc + c;
-    const bool last = w.seg == p.segs - 1;
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const bool in = lc + c < w.nc && n0 + m < p.dstate;
-      a[m] = in ? ld_any(p.A.ptr, static_cast<int64_t>(ch) * p.dstate + n0 + m, p.A.dtype) * kLog2e : 0.0f;
-      v[m] = 0.0f;
-      if (in && last && p.dfinal.ptr != nullptr)
-        v[m] = ld_any(p.dfinal.ptr, (static_cast<int64_t>(w.b) * p.dim + ch) * p.dstate + n0 + m, p.dfinal.dtype);
-      if (in && !last) v[m] = p.seg_state[(row_bs * p.dim + ch) * NP + n0 + m];
-    }
-    A2[c][0] = make_float2(a[0], a[1]), A2[c][1] = make_float2(a[2], a[3]);
-    g[c][0] = make_float2(v[0], v[1]), g[c][1] = make_float2(v[2], v[3]);
-    dA[c][0] = dA[c][1] = make_float2(0.f, 0.f);
-  }
-
-  const bool has_z = p.z.ptr != nullptr;
-  const int64_t kept_tiles = (p.seqlen + kSsmTile - 1) / kSsmTile;
-  // Element-wise mapping: vector k of a thread is channels ec.. of token row k; the column is the
-  // same for every k, so that a thread's channels are.
-  const int ec = (tid % VR) * 8, en = min(8, w.nc - ec);
-  auto row_of = [&](int k) { return (tid + k * kThreads) / VR; };
-  const T* const src[4] = {static_cast<const T*>(p.x.ptr) + w.b * p.x.sb + w.c0 + ec,
-                           static_cast<const T*>(p.dt.ptr) + w.b * p.dt.sb + w.c0 + ec,
-                           static_cast<const T*>(p.z.ptr) + w.b * p.z.sb + w.c0 + ec,
-                           static_cast<const T*>(p.dout.ptr) + w.b * p.dout.sb + w.c0 + ec};
-  const int64_t step[4] = {p.x.st, p.dt.st, p.z.st, p.dout.st};
-  const int vec[4] = {p.x.vec, p.dt.vec, p.z.vec, p.dout.vec};
-  const T* bp = static_cast<const T*>(p.Bm.ptr) + w.b * p.Bm.sb + w.g * p.Bm.sg;
-  const T* cp = static_cast<const T*>(p.Cm.ptr) + w.b * p.Cm.sb + w.g * p.Cm.sg;
-
-  auto fetch = [&](int t, int buf) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int r = row_of(k);
-      if (r < kTokens && en > 0 && t + r < w.t1) {
+    auto fetch = [&](int it, int ring) {
+      const int t = w.t0 + (tiles - 1 - it) * kTokens;
+      if (work && t + er < w.t1) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (i != 2 || has_z) copy_raw8(&s.raw[buf][i][k][0][tid], src[i] + static_cast<int64_t>(t + r) * step[i], en, vec[i], kThreads);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-
-  const int tiles = (w.t1 - w.t0 + kTokens - 1) / kTokens;
-  fetch(w.t0 + (tiles - 1) * kTokens, 0);
-  __syncthreads();  // sk
-
-  for (int it = tiles - 1; it >= 0; --it) {
-    const int t = w.t0 + it * kTokens, buf = (tiles - 1 - it) & 1;
-    const SeqBits seq = SEQ ? seq_bits(p, w.b, t) : SeqBits{0u, 0u, 0u};
-    float4 kept[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      kept[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (lc + c < w.nc) {
-        const int64_t kt = static_cast<int64_t>(w.b) * kept_tiles + t / kSsmTile;
-        kept[c] = *reinterpret_cast<const float4*>(p.kept + (kt * p.dim + w.c0 + lc + c) * NP + n0);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < NQ; ++k) {
-      const int i = tid + k * kThreads, tq = (i % QUADS) / NL, nq = 4 * (i % NL);
-      const int64_t tk = t + tq;
-      float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (tk < w.t1 && !(SEQ && ((seq.pad >> tq) & 1u)))
-        q = i < QUADS ? load4(bp + tk * p.Bm.st, nq, p.dstate, p.Bm.vec) : load4(cp + tk * p.Cm.st, nq, p.dstate, p.Cm.vec);
-      s.bc[i / QUADS][tq][i % NL] = q;
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int r = row_of(k);
-      if (r < kTokens) {
-        float x[8], d[8], z[8], o[8];
-        read_raw8<T>(&s.raw[buf][0][k][0][tid], kThreads, x);
-        read_raw8<T>(&s.raw[buf][1][k][0][tid], kThreads, d);
-        read_raw8<T>(&s.raw[buf][3][k][0][tid], kThreads, o);
-        const bool in = en > 0 && t + r < w.t1 && !(SEQ && ((seq.pad >> r) & 1u));
-        if (has_z) {
-          read_raw8<T>(&s.raw[buf][2][k][0][tid], kThreads, z);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] *= z[i] * sigmoid(z[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float raw = d[i] + s.sk[1][ec + i];
-          const float delta = p.softplus ? softplus(raw) : raw;
-          d[i] = in ? delta : 0.0f, x[i] = in ? delta * x[i] : 0.0f, o[i] = in ? o[i] : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-          *reinterpret_cast<float4*>(&s.f[0][r][ec + i]) = make_float4(d[i], d[i + 1], d[i + 2], d[i + 3]);
-          *reinterpret_cast<float4*>(&s.f[1][r][ec + i]) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-          *reinterpret_cast<float4*>(&s.f[2][r][ec + i]) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        }
-      }
-    }
-    __syncthreads();
-    if (it > 0) fetch(t - kTokens, buf ^ 1);
-
-    // One step of the recurrence; `a` gets the decays.
-    auto advance = [&](int i, float2 (&h)[4][2], float2 (&a)[4][2]) {
-      const float4 d4 = *reinterpret_cast<const float4*>(&s.f[0][i][lc]), u4 = *reinterpret_cast<const float4*>(&s.f[1][i][lc]);
-      const float4 b = s.bc[0][i][nl];
-      float d[4] = {d4.x, d4.y, d4.z, d4.w};
-      const float u[4] = {u4.x, u4.y, u4.z, u4.w};
-      const float2 B[2] = {make_float2(b.x, b.y), make_float2(b.z, b.w)};
-      if (SEQ && ((seq.start >> i) & 1u)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) d[c] = 0.0f, h[c][0] = h[c][1] = make_float2(0.f, 0.f);
+          if (i != 2 || has_z) copy8(&s.raw[ring][i][0][tid], src[i] + static_cast<int64_t>(t + er) * step[i], en, vec[i], kSsmHalf);
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          a[c][m] = exp2_approx2(fmul2(splat(d[c]), A2[c][m]));
-          h[c][m] = ffma2(a[c][m], h[c][m], fmul2(splat(u[c]), B[m]));
+      for (int k = 0; k < NQ; ++k) {
+        const int i = tid + k * kSsmHalf, nq = 4 * (i % NL);
+        const int64_t tk = t + (i % QUADS) / NL;
+        if (tk < w.t1) {
+          if (i < QUADS) copy4(&s.raw_bc[it & 1][k][tid], bp + tk * p.Bm.st, nq, p.dstate, p.Bm.vec);
+          else copy4(&s.raw_bc[it & 1][k][tid], cp + tk * p.Cm.st, nq, p.dstate, p.Cm.vec);
         }
+      }
+      if (SEQ) copy_ids(ids[it & 1], p, w.b, t);
+      copies_issued();
     };
+    fetch(0, 0);
 
-    {
-      float2 h[4][2], a[4][2];
+    float sums[2][8];  // dD and ddt_bias of the thread's channels
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s.h[0][c][tid] = kept[c];
-        h[c][0] = make_float2(kept[c].x, kept[c].y), h[c][1] = make_float2(kept[c].z, kept[c].w);
-      }
-#pragma unroll 1
-      for (int r = 1; r < kTokens / kRun; ++r) {
+    for (int i = 0; i < 8; ++i) sums[0][i] = sums[1][i] = 0.0f;
+    uint32_t off0 = 0, off1 = 0, off2 = 0;
+    int ring = 0;
+    for (int it = 0; it < tiles + 2; ++it, ring = next_stage(ring)) {
+      const int buf = it & 1;
+      off2 = off1, off1 = off0;
+      if (it >= 2) {
+        const int t = w.t0 + (tiles + 1 - it) * kTokens, old = next_stage(ring);  // two tiles ago
+        take_over(done_barrier(buf));
+        if (work && t + er < w.t1) {
+          const bool off = SEQ && ((off2 >> er) & 1u);
+          const int64_t at = (static_cast<int64_t>(w.b) * p.seqlen + t + er) * p.dim + w.c0 + ec;
+          const bool out_vec = (p.dim * sizeof(T)) % 16 == 0 && (w.c0 * sizeof(T)) % 16 == 0;
+          float x[8], o[8], v[8];
+          unpack8(read8<T>(&s.raw[old][0][0][tid], kSsmHalf), x);
+          unpack8(read8<T>(&s.raw[old][3][0][tid], kSsmHalf), o);
+          if (has_z) {
+            float z[8];
+            unpack8(read8<T>(&s.raw[old][2][0][tid], kSsmHalf), z);
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) advance((r - 1) * kRun + j, h, a);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s.h[r][c][tid] = make_float4(h[c][0].x, h[c][0].y, h[c][1].x, h[c][1].y);
-      }
-    }
-
-#pragma unroll 1
-    for (int r = kTokens / kRun - 1; r >= 0; --r) {
-      float2 h[kRun + 1][4][2], a[kRun][4][2];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float4 q = s.h[r][c][tid];
-        h[0][c][0] = make_float2(q.x, q.y), h[0][c][1] = make_float2(q.z, q.w);
-      }
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) h[j + 1][c][0] = h[j][c][0], h[j + 1][c][1] = h[j][c][1];
-        advance(r * kRun + j, h[j + 1], a[j]);
-      }
-#pragma unroll
-      for (int j = kRun - 1; j >= 0; --j) {
-        const int i = r * kRun + j;
-        const float4 d4 = *reinterpret_cast<const float4*>(&s.f[0][i][lc]), u4 = *reinterpret_cast<const float4*>(&s.f[1][i][lc]);
-        const float4 o4 = *reinterpret_cast<const float4*>(&s.f[2][i][lc]), b4 = s.bc[0][i][nl], c4 = s.bc[1][i][nl];
-        const float d[4] = {d4.x, d4.y, d4.z, d4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w}, o[4] = {o4.x, o4.y, o4.z, o4.w};
-        const float2 B[2] = {make_float2(b4.x, b4.y), make_float2(b4.z, b4.w)};
-        const float2 C[2] = {make_float2(c4.x, c4.y), make_float2(c4.z, c4.w)};
-        const bool start = SEQ && ((seq.start >> i) & 1u);
-        float2 dB[2], dC[2];
-        float v[12];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) dB[m] = dC[m] = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float2 y = make_float2(0.f, 0.f), gb = y, qa = y;
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const float2 gt = ffma2(splat(o[c]), C[m], g[c][m]), ht = h[j + 1][c][m];
-            y = ffma2(ht, C[m], y);
-            dC[m] = ffma2(splat(o[c]), ht, dC[m]);
-            dB[m] = ffma2(splat(u[c]), gt, dB[m]);
-            gb = ffma2(gt, B[m], gb);
-            float2 back = fmul2(a[j][c][m], gt);  // what the token before receives
-            float2 q = fmul2(back, h[j][c][m]);
-            if (start) back = q = make_float2(0.f, 0.f);
-            qa = ffma2(q, A2[c][m], qa);
-            dA[c][m] = ffma2(q, splat(d[c]), dA[c][m]);
-            g[c][m] = back;
+            for (int i = 0; i < 8; ++i) {
+              const float sg = sigmoid(z[i]), yt = fmaf(s.sk[0][ec + i], x[i], s.f[buf][0][er][ec + i]);
+              v[i] = off ? 0.0f : o[i] * yt * sg * fmaf(z[i], 1.0f - sg, 1.0f);  // dz
+              o[i] *= z[i] * sg;                                                  // dy
+            }
+            store8(static_cast<T*>(p.dz) + at, v, en, out_vec);
           }
-          v[3 * c] = y.x + y.y, v[3 * c + 1] = gb.x + gb.y, v[3 * c + 2] = qa.x + qa.y;
-        }
-        lane_sums<12, NL, 1>(v);
-        static_assert(share_size<12, NL>() == 3, "each of four lanes gets one channel's three sums");
-        __syncwarp();  // every lane has read token i's delta, delta x and dy
-        if (nl < 4) {
-          const int c = lc + lane_share<12, NL, 1>() / 3;
-          s.f[0][i][c] = v[0], s.f[1][i][c] = v[1], s.f[2][i][c] = v[2];
-        }
-        float e[8] = {dB[0].x, dB[0].y, dB[1].x, dB[1].y, dC[0].x, dC[0].y, dC[1].x, dC[1].y};
-        lane_sums<8, CL, NL>(e);
-        const int first = lane_share<8, CL, NL>();
-#pragma unroll
-        for (int k = 0; k < share_size<8, CL>(); ++k)
-          s.dbc[warp][i][((first + k) >> 2) * NP + n0 + ((first + k) & 3)] = e[k];
-      }
-    }
-    __syncthreads();
-
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int r = row_of(k);
-      if (r < kTokens && en > 0 && t + r < w.t1) {
-        float x[8], d[8], z[8], o[8], y[8], gb[8], qa[8];
-        read_raw8<T>(&s.raw[buf][0][k][0][tid], kThreads, x);
-        read_raw8<T>(&s.raw[buf][1][k][0][tid], kThreads, d);
-        read_raw8<T>(&s.raw[buf][3][k][0][tid], kThreads, o);
-#pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-          *reinterpret_cast<float4*>(&y[i]) = *reinterpret_cast<const float4*>(&s.f[0][r][ec + i]);
-          *reinterpret_cast<float4*>(&gb[i]) = *reinterpret_cast<const float4*>(&s.f[1][r][ec + i]);
-          *reinterpret_cast<float4*>(&qa[i]) = *reinterpret_cast<const float4*>(&s.f[2][r][ec + i]);
-        }
-        const bool off = SEQ && ((seq.pad >> r) & 1u);
-        const int64_t at = (static_cast<int64_t>(w.b) * p.seqlen + t + r) * p.dim + w.c0 + ec;
-        const bool out_vec = (p.dim * sizeof(T)) % 16 == 0 && (w.c0 * sizeof(T)) % 16 == 0;
-        if (has_z) {
-          read_raw8<T>(&s.raw[buf][2][k][0][tid], kThreads, z);
+          float dx[8], d[8];
+          unpack8(read8<T>(&s.raw[old][1][0][tid], kSsmHalf), d);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float sg = sigmoid(z[i]), yt = fmaf(s.sk[0][ec + i], x[i], y[i]);
-            y[i] = off ? 0.0f : o[i] * yt * sg * fmaf(z[i], 1.0f - sg, 1.0f);  // dz
-            o[i] *= z[i] * sg;                                                  // dy
+            const float gb = s.f[buf][1][er][ec + i], qa = s.f[buf][2][er][ec + i];
+            const float4 du = s.du[buf][er][(ec >> 1) + ((i >> 1) ^ (ec >> 4 & 3))];
+            const float delta = i % 2 ? du.y : du.x;
+            const float slope = p.softplus ? sigmoid(d[i] + s.sk[1][ec + i]) : 1.0f;
+            v[i] = off ? 0.0f : slope * fmaf(x[i], gb, kLn2 * qa);
+            dx[i] = off ? 0.0f : fmaf(delta, gb, s.sk[0][ec + i] * o[i]);
+            sums[0][i] += off ? 0.0f : o[i] * x[i];
+            sums[1][i] += v[i];
           }
-          store8(static_cast<T*>(p.dz) + at, y, en, out_vec);
+          store8(static_cast<T*>(p.dx) + at, dx, en, out_vec);
+          store8(static_cast<T*>(p.ddt) + at, v, en, out_vec);
+        }
+        const int64_t tok = static_cast<int64_t>(w.b) * p.seqlen + t;
+        for (int i = tid; i < kTokens * 2 * NP; i += kSsmHalf) {
+          const int r = i / (2 * NP), k = i % (2 * NP);
+          if (t + r < w.t1) {
+            const float v = (s.dbc[buf][0][r][k] + s.dbc[buf][1][r][k]) + (s.dbc[buf][2][r][k] + s.dbc[buf][3][r][k]);
+            p.part_bc[(((tok + r) * p.groups + w.g) * p.blocks + w.blk) * (2 * NP) + k] = v;
+          }
+        }
+      }
+      if (it < tiles) {
+        const int t = w.t0 + (tiles - 1 - it) * kTokens;
+        copies_done<0>();
+        SeqBits seq{0u, 0u, 0u};
+        if (SEQ) seq = seq_bits(*ids[buf], p, t);
+        off0 = seq.pad;
+        if (er < kTokens) {
+          float x[8], d[8], o[8];
+          unpack8(read8<T>(&s.raw[ring][0][0][tid], kSsmHalf), x);
+          unpack8(read8<T>(&s.raw[ring][1][0][tid], kSsmHalf), d);
+          unpack8(read8<T>(&s.raw[ring][3][0][tid], kSsmHalf), o);
+          // Padding takes no step and has no input; neither has what lies outside the piece.
+          const bool in = work && t + er < w.t1 && !(SEQ && ((seq.pad >> er) & 1u));
+          if (has_z) {
+            float z[8];
+            unpack8(read8<T>(&s.raw[ring][2][0][tid], kSsmHalf), z);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] *= z[i] * sigmoid(z[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; i += 4)
+            *reinterpret_cast<float4*>(&s.f[buf][0][er][ec + i]) =
+                in ? make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float2 delta = fadd2(make_float2(d[2 * i], d[2 * i + 1]), make_float2(s.sk[1][ec + 2 * i], s.sk[1][ec + 2 * i + 1]));
+            if (p.softplus) delta = softplus2(delta);
+            const float2 u = fmul2(delta, make_float2(x[2 * i], x[2 * i + 1]));
+            // A pair's place within its vector is turned as in the forward.
+            s.du[buf][er][(ec >> 1) + (i ^ (ec >> 4 & 3))] =
+                in ? make_float4(delta.x, delta.y, u.x, u.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float raw = d[i] + s.sk[1][ec + i];
-          float delta = raw, slope = 1.0f;
-          if (p.softplus) delta = softplus(raw), slope = sigmoid(raw);
-          const float dd = off ? 0.0f : slope * fmaf(x[i], gb[i], kLn2 * qa[i]);
-          s.sum[i][tid] += off ? 0.0f : o[i] * x[i];
-          s.sum[8 + i][tid] += dd;
-          x[i] = off ? 0.0f : fmaf(delta, gb[i], s.sk[0][ec + i] * o[i]);
-          d[i] = dd;
+        for (int k = 0; k < NQ; ++k) {
+          const int i = tid + k * kSsmHalf, tq = (i % QUADS) / NL;
+          const bool in = t + tq < w.t1 && !(SEQ && ((seq.pad >> tq) & 1u));
+          s.bc[buf][i / QUADS][tq][i % NL] = in ? unpack4(s.raw_bc[buf][k][tid]) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        store8(static_cast<T*>(p.dx) + at, x, en, out_vec);
-        store8(static_cast<T*>(p.ddt) + at, d, en, out_vec);
+        if (SEQ && tid == 0) s.start[buf] = seq.start;
+        hand_over(full_barrier(buf));
+        if (it + 1 < tiles) fetch(it + 1, next_stage(ring));
       }
     }
-    const int64_t tok = static_cast<int64_t>(w.b) * p.seqlen + t;
-    for (int i = tid; i < kTokens * 2 * NP; i += kThreads) {
-      const int r = i / (2 * NP), k = i % (2 * NP);
-      if (t + r < w.t1) {
-        const float v = (s.dbc[0][r][k] + s.dbc[1][r][k]) + (s.dbc[2][r][k] + s.dbc[3][r][k]);
-        p.part_bc[(((tok + r) * p.groups + w.g) * p.blocks + w.blk) * (2 * NP) + k] = v;
+
+    // dD and ddt_bias of the CTA: over the threads of one column of vectors, in order. The walk is done
+    // with the buffers (the last tile was taken over).
+    float* col = &s.f[0][0][0][0];
+    static_assert(sizeof(s.f) >= 8 * kSsmHalf * sizeof(float), "room for 8 values of each thread");
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      named_sync(7, kSsmHalf);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) col[i * kSsmHalf + tid] = sums[k][i];
+      named_sync(7, kSsmHalf);
+      for (int c = tid; c < w.nc; c += kSsmHalf) {
+        float v = 0.0f;
+        for (int q = c / 8; q < kSsmHalf; q += VR) v += col[(c % 8) * kSsmHalf + q];
+        p.part_d[((static_cast<int64_t>(w.b) * p.segs + w.seg) * 2 + k) * p.dim + w.c0 + c] = v;
       }
     }
   }
 
+  static __device__ __forceinline__ void walk(const SsmParams& p, const SsmPlace& w, S& s, int tiles) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int nl = lane % NL, n0 = 4 * nl;
+    const int pair = warp * CL + lane / NL, lc = 2 * pair;           // the lane's channel pair, its first channel within the block
+    const int place = (pair & ~3) | ((pair & 3) ^ (pair >> 3 & 3));  // of its du
+    const int64_t row_bs = static_cast<int64_t>(w.b) * p.segs + w.seg;
+    const int64_t kept_tiles = (p.seqlen + kSsmTile - 1) / kSsmTile;
+
+    // The lane's states before the tile at t, as the forward kept them.
+    auto fetch = [&](int t, int buf) {
+      const int64_t kt = static_cast<int64_t>(w.b) * kept_tiles + t / kSsmTile;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int ch = w.c0 + lc + c;
-    if (lc + c < w.nc) {
-      *reinterpret_cast<float4*>(p.part_a + (row_bs * p.dim + ch) * NP + n0) =
-          make_float4(dA[c][0].x, dA[c][0].y, dA[c][1].x, dA[c][1].y);
-      if (p.dinit != nullptr && w.seg == 0) {
-        const float v[4] = {g[c][0].x, g[c][0].y, g[c][1].x, g[c][1].y};
+      for (int c = 0; c < 2; ++c) {
+        if (lc + c < w.nc)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&s.kept[buf][c][tid])),
+                       "l"(p.kept + (kt * p.dim + w.c0 + lc + c) * NP + n0)
+                       : "memory");
+        else
+          s.kept[buf][c][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      copies_issued();
+    };
+    fetch(w.t0 + (tiles - 1) * kTokens, 0);
+
+    float2 A2[2][2], g[2][2], dA[2][2];
+    const bool last = w.seg == p.segs - 1;
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-          if (n0 + m < p.dstate)
-            st_any(p.dinit, (static_cast<int64_t>(w.b) * p.dim + ch) * p.dstate + n0 + m, p.init.dtype, v[m]);
+    for (int c = 0; c < 2; ++c) {
+      float a[4], v[4];
+      const int ch = w.c0 + lc + c;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const bool in = lc + c < w.nc && n0 + m < p.dstate;
+        a[m] = in ? ld_any(p.A.ptr, static_cast<int64_t>(ch) * p.dstate + n0 + m, p.A.dtype) * kLog2e : 0.0f;
+        v[m] = 0.0f;
+        if (in && last && p.dfinal.ptr != nullptr)
+          v[m] = ld_any(p.dfinal.ptr, (static_cast<int64_t>(w.b) * p.dim + ch) * p.dstate + n0 + m, p.dfinal.dtype);
+        if (in && !last) v[m] = p.seg_in[(row_bs * p.dim + ch) * NP + n0 + m];
+      }
+      A2[c][0] = make_float2(a[0], a[1]), A2[c][1] = make_float2(a[2], a[3]);
+      g[c][0] = make_float2(v[0], v[1]), g[c][1] = make_float2(v[2], v[3]);
+      dA[c][0] = dA[c][1] = make_float2(0.f, 0.f);
+    }
+
+#pragma unroll 1
+    for (int it = 0; it < tiles; ++it) {
+      const int t = w.t0 + (tiles - 1 - it) * kTokens, buf = it & 1;
+      if (it + 1 < tiles) fetch(t - kTokens, buf ^ 1);
+      else copies_issued();
+      copies_done<1>();
+      take_over(full_barrier(buf));
+      const uint32_t starts = SEQ ? s.start[buf] : 0u;
+
+      // One step of the recurrence; `a` gets the decays.
+      auto advance = [&](int i, float2 (&h)[2][2], float2 (&a)[2][2]) {
+        const float4 e = s.du[buf][i][place], b = s.bc[buf][0][i][nl];
+        float d[2] = {e.x, e.y};
+        const float u[2] = {e.z, e.w};
+        const float2 B[2] = {make_float2(b.x, b.y), make_float2(b.z, b.w)};
+        if (SEQ && ((starts >> i) & 1u)) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) d[c] = 0.0f, h[c][0] = h[c][1] = make_float2(0.f, 0.f);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            a[c][m] = exp2_approx2(fmul2(splat(d[c]), A2[c][m]));
+            h[c][m] = ffma2(a[c][m], h[c][m], fmul2(splat(u[c]), B[m]));
+          }
+      };
+      // The states before run r.
+      auto get = [&](int r, float2 (&h)[2][2]) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float4 q = r == 0 ? s.kept[buf][c][tid] : s.h[r - 1][c][tid];
+          h[c][0] = make_float2(q.x, q.y), h[c][1] = make_float2(q.z, q.w);
+        }
+      };
+
+      {
+        float2 h[2][2], a[2][2];
+        get(0, h);
+#pragma unroll 1
+        for (int r = 1; r < kTokens / kRun; ++r) {
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) advance((r - 1) * kRun + j, h, a);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) s.h[r - 1][c][tid] = make_float4(h[c][0].x, h[c][0].y, h[c][1].x, h[c][1].y);
+        }
+      }
+
+#pragma unroll 1
+      for (int r = kTokens / kRun - 1; r >= 0; --r) {
+        float2 h[kRun + 1][2][2], a[kRun][2][2];
+        get(r, h[0]);
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) h[j + 1][c][0] = h[j][c][0], h[j + 1][c][1] = h[j][c][1];
+          advance(r * kRun + j, h[j + 1], a[j]);
+        }
+        float v[kRun / 2][12];  // [two tokens][token, channel, (y, sum g B, sum q A)]
+        float e[kRun][8];       // dB, dC
+#pragma unroll
+        for (int j = kRun - 1; j >= 0; --j) {
+          const int i = r * kRun + j;
+          const float4 e4 = s.du[buf][i][place], b4 = s.bc[buf][0][i][nl], c4 = s.bc[buf][1][i][nl];
+          const float2 o2 = *reinterpret_cast<const float2*>(&s.f[buf][0][i][lc]);
+          const float d[2] = {e4.x, e4.y}, u[2] = {e4.z, e4.w}, o[2] = {o2.x, o2.y};
+          const float2 B[2] = {make_float2(b4.x, b4.y), make_float2(b4.z, b4.w)};
+          const float2 C[2] = {make_float2(c4.x, c4.y), make_float2(c4.z, c4.w)};
+          const bool start = SEQ && ((starts >> i) & 1u);
+          float2 dB[2], dC[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float2 y, gb, qa;
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              const float2 gt = ffma2(splat(o[c]), C[m], g[c][m]), ht = h[j + 1][c][m];
+              y = m ? ffma2(ht, C[m], y) : fmul2(ht, C[m]);
+              gb = m ? ffma2(gt, B[m], gb) : fmul2(gt, B[m]);
+              dC[m] = c ? ffma2(splat(o[c]), ht, dC[m]) : fmul2(splat(o[c]), ht);
+              dB[m] = c ? ffma2(splat(u[c]), gt, dB[m]) : fmul2(splat(u[c]), gt);
+              float2 back = fmul2(a[j][c][m], gt);  // what the token before receives
+              float2 q = fmul2(back, h[j][c][m]);
+              if (start) back = q = make_float2(0.f, 0.f);
+              qa = m ? ffma2(q, A2[c][m], qa) : fmul2(q, A2[c][m]);
+              dA[c][m] = ffma2(q, splat(d[c]), dA[c][m]);
+              g[c][m] = back;
+            }
+            float* vv = &v[j / 2][6 * (j % 2) + 3 * c];
+            vv[0] = y.x + y.y, vv[1] = gb.x + gb.y, vv[2] = qa.x + qa.y;
+          }
+          e[j][0] = dB[0].x, e[j][1] = dB[0].y, e[j][2] = dB[1].x, e[j][3] = dB[1].y;
+          e[j][4] = dC[0].x, e[j][5] = dC[0].y, e[j][6] = dC[1].x, e[j][7] = dC[1].y;
+          lane_sums<8, CL, NL>(e[j]);
+          if (j % 2 == 0) lane_sums<12, NL, 1>(v[j / 2]);
+        }
+        static_assert(share_size<12, NL>() == 3, "each of four lanes gets three sums of a token's channel");
+        __syncwarp();  // every lane has read the run's dy
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          const int i = r * kRun + j, first = lane_share<8, CL, NL>();
+#pragma unroll
+          for (int k = 0; k < share_size<8, CL>(); ++k)
+            s.dbc[buf][warp][i][((first + k) >> 2) * NP + n0 + ((first + k) & 3)] = e[j][k];
+          if (j % 2 == 0 && nl < 4) {
+            const int at = lane_share<12, NL, 1>() / 3;
+            s.f[buf][0][i + at / 2][lc + at % 2] = v[j / 2][0];
+            s.f[buf][1][i + at / 2][lc + at % 2] = v[j / 2][1];
+            s.f[buf][2][i + at / 2][lc + at % 2] = v[j / 2][2];
+          }
+        }
+      }
+      hand_over(done_barrier(buf));
+    }
+
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int ch = w.c0 + lc + c;
+      if (lc + c < w.nc) {
+        *reinterpret_cast<float4*>(p.part_a + (row_bs * p.dim + ch) * NP + n0) =
+            make_float4(dA[c][0].x, dA[c][0].y, dA[c][1].x, dA[c][1].y);
+        if (p.dinit != nullptr && w.seg == 0) {
+          const float v[4] = {g[c][0].x, g[c][0].y, g[c][1].x, g[c][1].y};
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            if (n0 + m < p.dstate)
+              st_any(p.dinit, (static_cast<int64_t>(w.b) * p.dim + ch) * p.dstate + n0 + m, p.init.dtype, v[m]);
+        }
       }
     }
   }
+};
+
+template <typename T, int NL, bool SEQ>
+__global__ void __launch_bounds__(kThreads, 2) cc1d_ssm_bwd_kernel(const __grid_constant__ SsmParams p) {
+  using K = Bwd<T, NL, SEQ>;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  typename K::S& s = *reinterpret_cast<typename K::S*>(smem_raw);
+  const SsmPlace w = ssm_place<K::CH>(p);
+  for (int i = threadIdx.x; i < 2 * K::CH; i += kThreads) {
+    const int c = i % K::CH;
+    const SsmParam& q = i < K::CH ? p.D : p.dt_bias;
+    s.sk[i / K::CH][c] = c < w.nc && q.ptr != nullptr ? ld_any(q.ptr, w.c0 + c, q.dtype) : 0.0f;
+  }
   __syncthreads();
-  for (int i = tid; i < 2 * CH; i += kThreads) {  // the threads of one column of vectors, in order
-    const int k = i / CH, c = i % CH;
-    if (c < w.nc) {
-      float v = 0.0f;
-      for (int q = c / 8; q < kThreads; q += VR) v += s.sum[8 * k + c % 8][q];
-      p.part_d[(row_bs * 2 + k) * p.dim + w.c0 + c] = v;
-    }
+  const int tiles = (w.t1 - w.t0 + kTokens - 1) / kTokens;
+  if (threadIdx.x < kSsmHalf) {
+    setmaxnreg_inc<kWalkRegs>();
+    K::walk(p, w, s, tiles);
+  } else {
+    setmaxnreg_dec<kElementRegs>();
+    K::elementwise(p, w, s, tiles);
   }
 }
 
@@ -407,8 +448,14 @@ template <typename T, int NL, bool SEQ>
 cudaError_t launch_main(const SsmParams& p, cudaStream_t s) {
   constexpr int smem = static_cast<int>(sizeof(BwdSmem<T, NL>));
   const auto kernel = cc1d_ssm_bwd_kernel<T, NL, SEQ>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
+  // setmaxnreg would wait for registers that a launch with fewer of them does not have.
+  static const bool holds_split = [&] {
+    cudaFuncAttributes a{};
+    return cudaFuncGetAttributes(&a, kernel) == cudaSuccess && 2 * a.numRegs >= kWalkRegs + kElementRegs;
+  }();
+  if (!holds_split) return cudaErrorLaunchOutOfResources;
   kernel<<<static_cast<unsigned>(p.batch) * p.segs * p.groups * p.blocks, kThreads, smem, s>>>(p);
   return cudaGetLastError();
 }

@@ -22,17 +22,19 @@ __device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
 // log(1 + exp(v)) = max(v, 0) + log1p(w) with w = exp(-|v|) in (0, 1]. log1p(w) = 2 atanh(s) with
 // s = w / (2 + w) <= 1/3, whose series 2 s (1 + s^2/3 + s^4/5 + ...) after seven terms is 3e-8 off
 // at most (s = 1/3) and keeps its relative accuracy as w goes to 0, where the step size is small.
-__device__ __forceinline__ float softplus(float v) {
-  const float w = __expf(-fabsf(v));
-  const float s = __fdividef(w, 2.0f + w), q = s * s;
-  float r = fmaf(q, 1.0f / 13, 1.0f / 11);
-  r = fmaf(r, q, 1.0f / 9);
-  r = fmaf(r, q, 1.0f / 7);
-  r = fmaf(r, q, 1.0f / 5);
-  r = fmaf(r, q, 1.0f / 3);
-  r = fmaf(r, q, 1.0f);
-  return fmaf(s + s, r, fmaxf(v, 0.0f));  // NaN: through s
+// A NaN comes through s.
+__device__ __forceinline__ float2 softplus2(float2 v) {
+  const float2 w = make_float2(__expf(-fabsf(v.x)), __expf(-fabsf(v.y)));
+  const float2 s = make_float2(__fdividef(w.x, 2.0f + w.x), __fdividef(w.y, 2.0f + w.y)), q = fmul2(s, s);
+  float2 r = ffma2(q, splat(1.0f / 13), splat(1.0f / 11));
+  r = ffma2(r, q, splat(1.0f / 9));
+  r = ffma2(r, q, splat(1.0f / 7));
+  r = ffma2(r, q, splat(1.0f / 5));
+  r = ffma2(r, q, splat(1.0f / 3));
+  r = ffma2(r, q, splat(1.0f));
+  return ffma2(fadd2(s, s), r, make_float2(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f)));
 }
+__device__ __forceinline__ float softplus(float v) { return softplus2(splat(v)).x; }
 
 __device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 
@@ -108,21 +110,91 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8], int n, bool 
   }
 }
 
-// States [n0, n0 + 4) of one token's B or C, zero at and beyond `n`.
+// States [n0, n0 + 4) of one token's B or C as loaded, zero at and beyond `n`.
 template <typename T>
-__device__ __forceinline__ float4 load4(const T* src, int n0, int n, bool vec) {
-  if (vec && n0 + 4 <= n) {
-    float2 f[2];
-    load_vec<T, 4>(src + n0, f);
-    return make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
-  }
-  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (n0 < n) r.x = to_f<T>(src[n0]);
-  if (n0 + 1 < n) r.y = to_f<T>(src[n0 + 1]);
-  if (n0 + 2 < n) r.z = to_f<T>(src[n0 + 2]);
-  if (n0 + 3 < n) r.w = to_f<T>(src[n0 + 3]);
+struct alignas(4 * sizeof(T)) Raw4 {
+  static constexpr int NW = static_cast<int>(sizeof(T));
+  uint32_t w[NW];
+};
+template <typename T>
+__device__ __forceinline__ Raw4<T> zero4() {
+  Raw4<T> r;
+#pragma unroll
+  for (int i = 0; i < Raw4<T>::NW; ++i) r.w[i] = 0u;
   return r;
 }
+template <typename T>
+__device__ __forceinline__ Raw4<T> load4(const T* src, int n0, int n, bool vec) {
+  Raw4<T> r;
+  if (vec && n0 + 4 <= n) {
+    if constexpr (sizeof(T) == 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(src + n0);
+      r.w[0] = q.x, r.w[1] = q.y, r.w[2] = q.z, r.w[3] = q.w;
+    } else {
+      const uint2 q = *reinterpret_cast<const uint2*>(src + n0);
+      r.w[0] = q.x, r.w[1] = q.y;
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = n0 + i < n ? reinterpret_cast<const uint32_t*>(src)[n0 + i] : 0u;
+  } else {
+    const uint16_t* s = reinterpret_cast<const uint16_t*>(src) + n0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t lo = n0 + 2 * i < n ? s[2 * i] : 0u, hi = n0 + 2 * i + 1 < n ? s[2 * i + 1] : 0u;
+      r.w[i] = lo | (hi << 16);
+    }
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float4 unpack4(const Raw4<T>& r) {
+  if constexpr (sizeof(T) == 4) {
+    return make_float4(__uint_as_float(r.w[0]), __uint_as_float(r.w[1]), __uint_as_float(r.w[2]), __uint_as_float(r.w[3]));
+  } else {
+    const float2 a = word_to_f2<T>(r.w[0]), b = word_to_f2<T>(r.w[1]);
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+}
+
+// The same two through shared memory, as asynchronous copies of the calling thread's own vectors where
+// these are aligned (each thread waits for and reads only its own). dst + i * stride is the vector's
+// i-th 16-byte piece.
+template <typename T>
+__device__ __forceinline__ void copy8(uint4* dst, const T* src, int n, bool vec, int stride) {
+  constexpr int Q = static_cast<int>(sizeof(T)) / 2;
+  if (vec && n == 8) {
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + i * stride)),
+                   "l"(reinterpret_cast<const uint4*>(src) + i)
+                   : "memory");
+  } else {
+    const Raw8<T> r = load8(src, n, false);
+#pragma unroll
+    for (int i = 0; i < Q; ++i) dst[i * stride] = make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> read8(const uint4* src, int stride) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < Raw8<T>::NW / 4; ++i) {
+    const uint4 q = src[i * stride];
+    r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void copy4(Raw4<T>* dst, const T* src, int n0, int n, bool vec) {
+  if (vec && n0 + 4 <= n)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src + n0), "n"(4 * sizeof(T)) : "memory");
+  else
+    *dst = load4(src, n0, n, false);
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>  // waits for all groups but the last N
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Sums v[0..V) over the L lanes of a warp that differ in lane bits BIT, 2 BIT, ... While the number
 // of values is even, a stage halves it: each lane sends the half that its partner keeps, so V values
@@ -173,6 +245,17 @@ constexpr int share_lanes() {
     return 1;
 }
 
+// A CTA's two halves, a walk and the element-wise work around it, hand tiles to each other in
+// kSsmStages buffers through two named barriers each: `full` (element-wise arrives, walk waits) and
+// `done` (the reverse). Both halves pass the same ones for the same tiles, so every wait ends.
+constexpr int kSsmHalf = 128;  // threads of each
+constexpr int kSsmStages = 3;
+__device__ __forceinline__ void hand_over(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(2 * kSsmHalf) : "memory"); }
+__device__ __forceinline__ void take_over(int id) { named_sync(id, 2 * kSsmHalf); }
+__device__ __forceinline__ int full_barrier(int stage) { return 1 + stage; }
+__device__ __forceinline__ int done_barrier(int stage) { return 1 + kSsmStages + stage; }
+__device__ __forceinline__ int next_stage(int stage) { return stage + 1 == kSsmStages ? 0 : stage + 1; }
+
 // What a CTA works on: batch row, piece of the sequence, group and its block of channels. The
 // channel blocks of one piece are neighbours in the grid, so that they share its B and C in L2.
 struct SsmPlace {
@@ -195,25 +278,34 @@ __device__ __forceinline__ SsmPlace ssm_place(const SsmParams& p) {
   return w;
 }
 
-// The 32 tokens from t (bit i: token t + i) of row b: those whose state starts from zero because the
-// sequence id differs from the token before (the row's first token continues initial_states),
-// the padding ones, and the last ones of their sequence.
+// Tokens of a tile (bit i: token t + i of row b) whose state starts from zero because the sequence id
+// differs from the token before (the row's first token continues initial_states), the padding ones,
+// and the last ones of their sequence. From lane i's ids of token t + i and its neighbours, loaded
+// early; whole warps call it.
+struct SeqIds {
+  int32_t prev, cur, next;
+};
 struct SeqBits {
   uint32_t start, pad, last;
 };
-__device__ __forceinline__ SeqBits seq_bits(const SsmParams& p, int b, int t) {
-  SeqBits r{0u, 0u, 0u};
-  if (p.seq_idx != nullptr) {
-    const int32_t* s = p.seq_idx + static_cast<int64_t>(b) * p.seqlen;
-    const int i = t + static_cast<int>(threadIdx.x & 31);
-    const bool in = i < p.seqlen;
-    const int cur = in ? s[i] : -1;
-    const int prev = in && i > 0 ? s[i - 1] : cur;
-    const int next = i + 1 < p.seqlen ? s[i + 1] : -1;
-    r.start = __ballot_sync(0xffffffffu, in && prev != cur);
-    r.pad = __ballot_sync(0xffffffffu, in && cur < 0);
-    r.last = __ballot_sync(0xffffffffu, in && cur >= 0 && (i + 1 == p.seqlen || next != cur));
+__device__ __forceinline__ void copy_ids(SeqIds* dst, const SsmParams& p, int b, int t) {
+  const int i = t + static_cast<int>(threadIdx.x & 31);
+  if ((threadIdx.x & 31) < kSsmTile && i < p.seqlen) {
+    const int32_t* s = p.seq_idx + static_cast<int64_t>(b) * p.seqlen + i;
+    const int32_t* from[3] = {i > 0 ? s - 1 : s, s, i + 1 < p.seqlen ? s + 1 : s};
+    int32_t* to[3] = {&dst->prev, &dst->cur, &dst->next};
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to[k])), "l"(from[k]) : "memory");
   }
+}
+__device__ __forceinline__ SeqBits seq_bits(const SeqIds& id, const SsmParams& p, int t) {
+  const int lane = threadIdx.x & 31, i = t + lane;
+  const bool in = lane < kSsmTile && i < p.seqlen;
+  SeqBits r;
+  r.start = __ballot_sync(0xffffffffu, in && id.prev != id.cur);
+  r.pad = __ballot_sync(0xffffffffu, in && id.cur < 0);
+  r.last = __ballot_sync(0xffffffffu, in && id.cur >= 0 && (i + 1 == p.seqlen || id.next != id.cur));
   return r;
 }
 
