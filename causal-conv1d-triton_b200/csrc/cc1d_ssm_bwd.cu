@@ -7,6 +7,8 @@
 //   dz = dout y silu'(z)                dD = sum_t dy x                  ddt = ddelta softplus'
 // It needs every h[t], which the forward does not keep: it keeps the state before each 16th token,
 // and the states between are computed again.
+#include <type_traits>
+
 #include "cc1d_ssm_device.cuh"
 
 namespace cc1d {
@@ -27,7 +29,8 @@ struct BwdSmem {
   // Handed over.
   float4 du[kBuffers][kTokens][CH / 2];          // (delta, delta, delta x, delta x) of a channel pair
   float f[kBuffers][3][kTokens][CH];             // dy, then sum C h; sum g B; sum q A
-  float4 bc[kBuffers][2][kTokens][NL];           // B, C
+  static constexpr int ORDERS = NL == 4 ? 2 : 1;  // above, a second copy would leave room for one CTA an SM only
+  float4 bc[kBuffers][2][kTokens][ORDERS][NL];   // B, C; and with their pairs of states exchanged
   float dbc[kBuffers][kWarps][kTokens][2 * NP];  // each warp's dB and dC of the tile
   uint32_t start[kBuffers];                      // SeqBits of the tile
   // The walk's own, private to a thread: states before each run but the first, and before the tile.
@@ -49,7 +52,9 @@ struct BwdSmem {
 // channels (dB, dC) are first formed inside the lane, then across lanes by lane_sums: 12 values of two
 // tokens over NL lanes, 8 of each token over the rest. A tile's states are first walked through,
 // keeping those before every 4th token, and each run of 4 tokens is then computed once more into
-// registers and walked back. All stores to shared memory of a run are at its end, so that nothing
+// registers and walked back. Half of the channel lanes hold their two pairs of states in exchanged
+// order: what a lane sends in the first stage of the dB and dC sums is then its second pair and what it
+// keeps its first, in every lane, without the selections that the other stages need. All stores to shared memory of a run are at its end, so that nothing
 // keeps the loads of its next token from being issued early.
 // SEQ: packed rows (seq_idx), where a step may have to drop what came before it.
 template <typename T, int NL, bool SEQ>
@@ -185,7 +190,9 @@ struct Bwd {
         for (int k = 0; k < NQ; ++k) {
           const int i = tid + k * kSsmHalf, tq = (i % QUADS) / NL;
           const bool in = t + tq < w.t1 && !(SEQ && ((seq.pad >> tq) & 1u));
-          s.bc[buf][i / QUADS][tq][i % NL] = in ? unpack4(s.raw_bc[buf][k][tid]) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 q = in ? unpack4(s.raw_bc[buf][k][tid]) : make_float4(0.f, 0.f, 0.f, 0.f);
+          s.bc[buf][i / QUADS][tq][0][i % NL] = q;
+          if (S::ORDERS == 2) s.bc[buf][i / QUADS][tq][S::ORDERS - 1][i % NL] = make_float4(q.z, q.w, q.x, q.y);
         }
         if (SEQ && tid == 0) s.start[buf] = seq.start;
         hand_over(full_barrier(buf));
@@ -211,11 +218,136 @@ struct Bwd {
     }
   }
 
+  // One tile of the walk. CUTS: a sequence starts in it (bits of `starts`).
+  template <typename Cuts>
+  static __device__ __forceinline__ void tile(S& s, int buf, uint32_t starts, const float2 (&A2)[2][2],
+                                              float2 (&g)[2][2], float2 (&dA)[2][2], Cuts) {
+    constexpr bool CUTS = Cuts::value;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nl = lane % NL;
+    const int pair = warp * CL + lane / NL, lc = 2 * pair, place = (pair & ~3) | ((pair & 3) ^ (pair >> 3 & 3));
+    const int turn = (lane & NL) ? 1 : 0;
+
+    // B (k = 0) or C of token i, the lane's first pair of states first.
+    auto four = [&](int k, int i, float2 (&v)[2]) {
+      if constexpr (S::ORDERS == 2) {
+        const float4 q = s.bc[buf][k][i][turn][nl];
+        v[0] = make_float2(q.x, q.y), v[1] = make_float2(q.z, q.w);
+      } else {
+        const float2* q = reinterpret_cast<const float2*>(&s.bc[buf][k][i][0][nl]);
+        v[0] = q[turn], v[1] = q[1 - turn];
+      }
+    };
+    // One step of the recurrence; `a` gets the decays.
+    auto advance = [&](int i, float2 (&h)[2][2], float2 (&a)[2][2]) {
+      const float4 e = s.du[buf][i][place];
+      float d[2] = {e.x, e.y};
+      const float u[2] = {e.z, e.w};
+      float2 B[2];
+      four(0, i, B);
+      if (CUTS && ((starts >> i) & 1u)) d[0] = d[1] = 0.0f, h[0][0] = h[0][1] = h[1][0] = h[1][1] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          a[c][m] = exp2_approx2(fmul2(splat(d[c]), A2[c][m]));
+          h[c][m] = ffma2(a[c][m], h[c][m], fmul2(splat(u[c]), B[m]));
+        }
+    };
+    // The states before run r.
+    auto get = [&](int r, float2 (&h)[2][2]) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float4 q = r == 0 ? s.kept[buf][c][tid] : s.h[r - 1][c][tid];
+        h[c][0] = make_float2(q.x, q.y), h[c][1] = make_float2(q.z, q.w);
+      }
+    };
+
+    {
+      float2 h[2][2], a[2][2];
+      get(0, h);
+#pragma unroll 1
+      for (int r = 1; r < kTokens / kRun; ++r) {
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) advance((r - 1) * kRun + j, h, a);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) s.h[r - 1][c][tid] = make_float4(h[c][0].x, h[c][0].y, h[c][1].x, h[c][1].y);
+      }
+    }
+
+#pragma unroll 1
+    for (int r = kTokens / kRun - 1; r >= 0; --r) {
+      float2 h[kRun + 1][2][2], a[kRun][2][2];
+      get(r, h[0]);
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) h[j + 1][c][0] = h[j][c][0], h[j + 1][c][1] = h[j][c][1];
+        advance(r * kRun + j, h[j + 1], a[j]);
+      }
+      float v[kRun / 2][12];  // [two tokens][token, channel, (y, sum g B, sum q A)]
+      float e[kRun][8];       // [pair of states][dB, dC][state]
+#pragma unroll
+      for (int j = kRun - 1; j >= 0; --j) {
+        const int i = r * kRun + j;
+        const float4 e4 = s.du[buf][i][place];
+        const float2 o2 = *reinterpret_cast<const float2*>(&s.f[buf][0][i][lc]);
+        const float d[2] = {e4.x, e4.y}, u[2] = {e4.z, e4.w}, o[2] = {o2.x, o2.y};
+        float2 B[2], C[2];
+        four(0, i, B), four(1, i, C);
+        const bool start = CUTS && ((starts >> i) & 1u);
+        float2 dB[2], dC[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float2 y, gb, qa;
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const float2 gt = ffma2(splat(o[c]), C[m], g[c][m]), ht = h[j + 1][c][m];
+            y = m ? ffma2(ht, C[m], y) : fmul2(ht, C[m]);
+            gb = m ? ffma2(gt, B[m], gb) : fmul2(gt, B[m]);
+            dC[m] = c ? ffma2(splat(o[c]), ht, dC[m]) : fmul2(splat(o[c]), ht);
+            dB[m] = c ? ffma2(splat(u[c]), gt, dB[m]) : fmul2(splat(u[c]), gt);
+            float2 back = fmul2(a[j][c][m], gt);  // what the token before receives
+            float2 q = fmul2(back, h[j][c][m]);
+            if (start) back = q = make_float2(0.f, 0.f);
+            qa = m ? ffma2(q, A2[c][m], qa) : fmul2(q, A2[c][m]);
+            dA[c][m] = ffma2(q, splat(d[c]), dA[c][m]);
+            g[c][m] = back;
+          }
+          float* vv = &v[j / 2][6 * (j % 2) + 3 * c];
+          vv[0] = y.x + y.y, vv[1] = gb.x + gb.y, vv[2] = qa.x + qa.y;
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          e[j][4 * m] = dB[m].x, e[j][4 * m + 1] = dB[m].y, e[j][4 * m + 2] = dC[m].x, e[j][4 * m + 3] = dC[m].y;
+        // The lane across NL holds the pairs the other way round: its second is this lane's first.
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[j][k] += __shfl_xor_sync(0xffffffffu, e[j][4 + k], NL);
+        lane_sums<4, CL / 2, 2 * NL>(e[j]);
+        if (j % 2 == 0) lane_sums<12, NL, 1>(v[j / 2]);
+      }
+      static_assert(share_size<12, NL>() == 3, "each of four lanes gets three sums of a token's channel");
+      __syncwarp();  // every lane has read the run's dy
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        const int i = r * kRun + j, first = lane_share<4, CL / 2, 2 * NL>();
+#pragma unroll
+        for (int k = 0; k < share_size<4, CL / 2>(); ++k)
+          s.dbc[buf][warp][i][((first + k) >> 1) * NP + 4 * nl + 2 * turn + ((first + k) & 1)] = e[j][k];
+        if (j % 2 == 0 && nl < 4) {
+          const int at = lane_share<12, NL, 1>() / 3;
+          s.f[buf][0][i + at / 2][lc + at % 2] = v[j / 2][0];
+          s.f[buf][1][i + at / 2][lc + at % 2] = v[j / 2][1];
+          s.f[buf][2][i + at / 2][lc + at % 2] = v[j / 2][2];
+        }
+      }
+    }
+  }
+
   static __device__ __forceinline__ void walk(const SsmParams& p, const SsmPlace& w, S& s, int tiles) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int nl = lane % NL, n0 = 4 * nl;
-    const int pair = warp * CL + lane / NL, lc = 2 * pair;           // the lane's channel pair, its first channel within the block
-    const int place = (pair & ~3) | ((pair & 3) ^ (pair >> 3 & 3));  // of its du
+    const int tid = threadIdx.x, lane = tid & 31, n0 = 4 * (lane % NL);
+    const int lc = 2 * ((tid >> 5) * CL + lane / NL);  // first of the lane's channels, within the block
+    const int turn = (lane & NL) ? 1 : 0, n1 = n0 + 2 * turn, n2 = n0 + 2 - 2 * turn;  // first state of either pair
+    auto state = [&](int m) { return (m < 2 ? n1 : n2) + (m & 1); };
     const int64_t row_bs = static_cast<int64_t>(w.b) * p.segs + w.seg;
     const int64_t kept_tiles = (p.seqlen + kSsmTile - 1) / kSsmTile;
 
@@ -225,9 +357,10 @@ struct Bwd {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if (lc + c < w.nc)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&s.kept[buf][c][tid])),
-                       "l"(p.kept + (kt * p.dim + w.c0 + lc + c) * NP + n0)
-                       : "memory");
+          for (int m = 0; m < 2; ++m)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(&s.kept[buf][c][tid]) + 8 * m),
+                         "l"(p.kept + (kt * p.dim + w.c0 + lc + c) * NP + state(2 * m))
+                         : "memory");
         else
           s.kept[buf][c][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
@@ -243,12 +376,13 @@ struct Bwd {
       const int ch = w.c0 + lc + c;
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        const bool in = lc + c < w.nc && n0 + m < p.dstate;
-        a[m] = in ? ld_any(p.A.ptr, static_cast<int64_t>(ch) * p.dstate + n0 + m, p.A.dtype) * kLog2e : 0.0f;
+        const int n = state(m);
+        const bool in = lc + c < w.nc && n < p.dstate;
+        a[m] = in ? ld_any(p.A.ptr, static_cast<int64_t>(ch) * p.dstate + n, p.A.dtype) * kLog2e : 0.0f;
         v[m] = 0.0f;
         if (in && last && p.dfinal.ptr != nullptr)
-          v[m] = ld_any(p.dfinal.ptr, (static_cast<int64_t>(w.b) * p.dim + ch) * p.dstate + n0 + m, p.dfinal.dtype);
-        if (in && !last) v[m] = p.seg_in[(row_bs * p.dim + ch) * NP + n0 + m];
+          v[m] = ld_any(p.dfinal.ptr, (static_cast<int64_t>(w.b) * p.dim + ch) * p.dstate + n, p.dfinal.dtype);
+        if (in && !last) v[m] = p.seg_in[(row_bs * p.dim + ch) * NP + n];
       }
       A2[c][0] = make_float2(a[0], a[1]), A2[c][1] = make_float2(a[2], a[3]);
       g[c][0] = make_float2(v[0], v[1]), g[c][1] = make_float2(v[2], v[3]);
@@ -263,109 +397,8 @@ struct Bwd {
       copies_done<1>();
       take_over(full_barrier(buf));
       const uint32_t starts = SEQ ? s.start[buf] : 0u;
-
-      // One step of the recurrence; `a` gets the decays.
-      auto advance = [&](int i, float2 (&h)[2][2], float2 (&a)[2][2]) {
-        const float4 e = s.du[buf][i][place], b = s.bc[buf][0][i][nl];
-        float d[2] = {e.x, e.y};
-        const float u[2] = {e.z, e.w};
-        const float2 B[2] = {make_float2(b.x, b.y), make_float2(b.z, b.w)};
-        if (SEQ && ((starts >> i) & 1u)) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) d[c] = 0.0f, h[c][0] = h[c][1] = make_float2(0.f, 0.f);
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            a[c][m] = exp2_approx2(fmul2(splat(d[c]), A2[c][m]));
-            h[c][m] = ffma2(a[c][m], h[c][m], fmul2(splat(u[c]), B[m]));
-          }
-      };
-      // The states before run r.
-      auto get = [&](int r, float2 (&h)[2][2]) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float4 q = r == 0 ? s.kept[buf][c][tid] : s.h[r - 1][c][tid];
-          h[c][0] = make_float2(q.x, q.y), h[c][1] = make_float2(q.z, q.w);
-        }
-      };
-
-      {
-        float2 h[2][2], a[2][2];
-        get(0, h);
-#pragma unroll 1
-        for (int r = 1; r < kTokens / kRun; ++r) {
-#pragma unroll
-          for (int j = 0; j < kRun; ++j) advance((r - 1) * kRun + j, h, a);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) s.h[r - 1][c][tid] = make_float4(h[c][0].x, h[c][0].y, h[c][1].x, h[c][1].y);
-        }
-      }
-
-#pragma unroll 1
-      for (int r = kTokens / kRun - 1; r >= 0; --r) {
-        float2 h[kRun + 1][2][2], a[kRun][2][2];
-        get(r, h[0]);
-#pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) h[j + 1][c][0] = h[j][c][0], h[j + 1][c][1] = h[j][c][1];
-          advance(r * kRun + j, h[j + 1], a[j]);
-        }
-        float v[kRun / 2][12];  // [two tokens][token, channel, (y, sum g B, sum q A)]
-        float e[kRun][8];       // dB, dC
-#pragma unroll
-        for (int j = kRun - 1; j >= 0; --j) {
-          const int i = r * kRun + j;
-          const float4 e4 = s.du[buf][i][place], b4 = s.bc[buf][0][i][nl], c4 = s.bc[buf][1][i][nl];
-          const float2 o2 = *reinterpret_cast<const float2*>(&s.f[buf][0][i][lc]);
-          const float d[2] = {e4.x, e4.y}, u[2] = {e4.z, e4.w}, o[2] = {o2.x, o2.y};
-          const float2 B[2] = {make_float2(b4.x, b4.y), make_float2(b4.z, b4.w)};
-          const float2 C[2] = {make_float2(c4.x, c4.y), make_float2(c4.z, c4.w)};
-          const bool start = SEQ && ((starts >> i) & 1u);
-          float2 dB[2], dC[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float2 y, gb, qa;
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              const float2 gt = ffma2(splat(o[c]), C[m], g[c][m]), ht = h[j + 1][c][m];
-              y = m ? ffma2(ht, C[m], y) : fmul2(ht, C[m]);
-              gb = m ? ffma2(gt, B[m], gb) : fmul2(gt, B[m]);
-              dC[m] = c ? ffma2(splat(o[c]), ht, dC[m]) : fmul2(splat(o[c]), ht);
-              dB[m] = c ? ffma2(splat(u[c]), gt, dB[m]) : fmul2(splat(u[c]), gt);
-              float2 back = fmul2(a[j][c][m], gt);  // what the token before receives
-              float2 q = fmul2(back, h[j][c][m]);
-              if (start) back = q = make_float2(0.f, 0.f);
-              qa = m ? ffma2(q, A2[c][m], qa) : fmul2(q, A2[c][m]);
-              dA[c][m] = ffma2(q, splat(d[c]), dA[c][m]);
-              g[c][m] = back;
-            }
-            float* vv = &v[j / 2][6 * (j % 2) + 3 * c];
-            vv[0] = y.x + y.y, vv[1] = gb.x + gb.y, vv[2] = qa.x + qa.y;
-          }
-          e[j][0] = dB[0].x, e[j][1] = dB[0].y, e[j][2] = dB[1].x, e[j][3] = dB[1].y;
-          e[j][4] = dC[0].x, e[j][5] = dC[0].y, e[j][6] = dC[1].x, e[j][7] = dC[1].y;
-          lane_sums<8, CL, NL>(e[j]);
-          if (j % 2 == 0) lane_sums<12, NL, 1>(v[j / 2]);
-        }
-        static_assert(share_size<12, NL>() == 3, "each of four lanes gets three sums of a token's channel");
-        __syncwarp();  // every lane has read the run's dy
-#pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-          const int i = r * kRun + j, first = lane_share<8, CL, NL>();
-#pragma unroll
-          for (int k = 0; k < share_size<8, CL>(); ++k)
-            s.dbc[buf][warp][i][((first + k) >> 2) * NP + n0 + ((first + k) & 3)] = e[j][k];
-          if (j % 2 == 0 && nl < 4) {
-            const int at = lane_share<12, NL, 1>() / 3;
-            s.f[buf][0][i + at / 2][lc + at % 2] = v[j / 2][0];
-            s.f[buf][1][i + at / 2][lc + at % 2] = v[j / 2][1];
-            s.f[buf][2][i + at / 2][lc + at % 2] = v[j / 2][2];
-          }
-        }
-      }
+      if (SEQ && starts != 0u) tile(s, buf, starts, A2, g, dA, std::true_type{});
+      else tile(s, buf, 0u, A2, g, dA, std::false_type{});
       hand_over(done_barrier(buf));
     }
 
@@ -373,14 +406,14 @@ struct Bwd {
     for (int c = 0; c < 2; ++c) {
       const int ch = w.c0 + lc + c;
       if (lc + c < w.nc) {
-        *reinterpret_cast<float4*>(p.part_a + (row_bs * p.dim + ch) * NP + n0) =
-            make_float4(dA[c][0].x, dA[c][0].y, dA[c][1].x, dA[c][1].y);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) *reinterpret_cast<float2*>(p.part_a + (row_bs * p.dim + ch) * NP + state(2 * m)) = dA[c][m];
         if (p.dinit != nullptr && w.seg == 0) {
           const float v[4] = {g[c][0].x, g[c][0].y, g[c][1].x, g[c][1].y};
 #pragma unroll
           for (int m = 0; m < 4; ++m)
-            if (n0 + m < p.dstate)
-              st_any(p.dinit, (static_cast<int64_t>(w.b) * p.dim + ch) * p.dstate + n0 + m, p.init.dtype, v[m]);
+            if (state(m) < p.dstate)
+              st_any(p.dinit, (static_cast<int64_t>(w.b) * p.dim + ch) * p.dstate + state(m), p.init.dtype, v[m]);
         }
       }
     }

@@ -1,6 +1,8 @@
 // Forward of the input-dependent state-space recurrence, per channel d and state n:
 //   h[t] = exp(delta[t] A[d, n]) h[t-1] + delta[t] x[t] B[t, n]
 //   out[t] = (sum_n C[t, n] h[t] + D[d] x[t]) silu(z[t]),   delta = softplus(dt + dt_bias)
+#include <type_traits>
+
 #include "cc1d_ssm_device.cuh"
 
 namespace cc1d {
@@ -207,7 +209,7 @@ struct Scan {
     for (int it = 0; it < tiles; ++it, buf = next_stage(buf)) {
       const int t = tile_start(w, tiles, it);
       take_over(full_barrier(buf));
-      const uint32_t starts = SEQ ? s.start[buf] : 0u, lasts = SEQ ? s.last[buf] : 0u;
+      const uint32_t starts = SEQ ? s.start[buf] : 0u, lasts = SEQ && p.cache != nullptr ? s.last[buf] : 0u;
       if constexpr (FWD) {
         if (p.kept != nullptr) {
           const int64_t kt = static_cast<int64_t>(w.b) * kept_tiles + t / kSsmTile;
@@ -218,47 +220,54 @@ struct Scan {
                   make_float4(h[c][0].x, h[c][0].y, h[c][1].x, h[c][1].y);
         }
       }
-      // The tile's sums are stored at its end, so that nothing keeps the loads and the exponentials of later
-      // tokens from being issued early.
+      // The tile's sums over states are stored at its end, so that nothing keeps the loads and the
+      // exponentials of later tokens from being issued early.
       float v[kTokens / 4][8];  // [four tokens][token, channel]
-#pragma unroll
-      for (int q = 0; q < kTokens; q += 4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = BACK ? kTokens - 1 - q - j : q + j;
-          const float4 e = s.du[buf][i][place], k4 = s.bc[buf][BACK ? 1 : 0][i][nl];
-          float delta[2] = {e.x, e.y};
-          const float u[2] = {e.z, e.w};
-          const float2 K[2] = {make_float2(k4.x, k4.y), make_float2(k4.z, k4.w)};
-          const bool start = SEQ && ((starts >> i) & 1u);
-          if (!BACK && start) {
-            cut = true;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) h[c][0] = h[c][1] = make_float2(0.f, 0.f), delta[c] = 0.0f;
-          }
+      // CUTS: a sequence starts or ends in the tile.
+      auto tokens = [&](auto cuts) {
+        constexpr bool CUTS = decltype(cuts)::value;
+        // The decays of a token are computed while the one before is worked on.
+        float2 a[2][2][2];
+        float4 e[2];
+        auto decays = [&](int k) {
+          const int i = BACK ? kTokens - 1 - k : k;
+          e[k & 1] = s.du[buf][i][place];
+          const bool start = !BACK && CUTS && ((starts >> i) & 1u);
+          const float d[2] = {start ? 0.0f : e[k & 1].x, start ? 0.0f : e[k & 1].y};
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              const float2 a = exp2_approx2(fmul2(splat(delta[c]), A2[c][m]));
-              if constexpr (BACK) h[c][m] = fmul2(a, ffma2(splat(u[c]), K[m], h[c][m]));
-              else h[c][m] = ffma2(a, h[c][m], fmul2(splat(u[c]), K[m]));
-            }
-            if constexpr (!FWD) sum_delta[c] += delta[c];
+            for (int m = 0; m < 2; ++m) a[k & 1][c][m] = exp2_approx2(fmul2(splat(d[c]), A2[c][m]));
+            if constexpr (!FWD) sum_delta[c] += d[c];
           }
-          if (BACK && start) {
-            cut = true;
+        };
+        decays(0);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) h[c][0] = h[c][1] = make_float2(0.f, 0.f);
-          }
+        for (int k = 0; k < kTokens; ++k) {
+          const int i = BACK ? kTokens - 1 - k : k;
+          if (k + 1 < kTokens) decays(k + 1);
+          const float4 k4 = s.bc[buf][BACK ? 1 : 0][i][nl];
+          const float u[2] = {e[k & 1].z, e[k & 1].w};
+          const float2 K[2] = {make_float2(k4.x, k4.y), make_float2(k4.z, k4.w)};
+          const bool start = CUTS && ((starts >> i) & 1u);
+          if (!BACK && start) h[0][0] = h[0][1] = h[1][0] = h[1][1] = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              if constexpr (BACK) h[c][m] = fmul2(a[k & 1][c][m], ffma2(splat(u[c]), K[m], h[c][m]));
+              else h[c][m] = ffma2(a[k & 1][c][m], h[c][m], fmul2(splat(u[c]), K[m]));
+            }
+          if (BACK && start) h[0][0] = h[0][1] = h[1][0] = h[1][1] = make_float2(0.f, 0.f);
           if constexpr (FWD) {
             const float4 c4 = s.bc[buf][1][i][nl];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               const float2 y = ffma2(h[c][1], make_float2(c4.z, c4.w), fmul2(h[c][0], make_float2(c4.x, c4.y)));
-              v[q / 4][2 * j + c] = y.x + y.y;
+              v[k / 4][2 * (k % 4) + c] = y.x + y.y;
             }
-            if (SEQ && p.cache != nullptr && ((lasts >> i) & 1u)) {
+            if (k % 4 == 3) lane_sums<8, NL, 1>(v[k / 4]);
+            if (CUTS && ((lasts >> i) & 1u)) {
               const int id = p.seq_idx[static_cast<int64_t>(w.b) * p.seqlen + t + i];
               const int64_t slot = id < p.cache_n ? p.cache_idx[w.b * p.cache_n + id] : -1;
               if (slot >= 0 && slot < p.cache_slots) {
@@ -274,16 +283,21 @@ struct Scan {
             }
           }
         }
-        if constexpr (FWD) lane_sums<8, NL, 1>(v[q / 4]);
+      };
+      if (SEQ && (starts | lasts) != 0u) {
+        cut = cut || starts != 0u;
+        tokens(std::true_type{});
+      } else {
+        tokens(std::false_type{});
       }
       if constexpr (FWD) {
         const int at = lane_share<8, NL, 1>();
 #pragma unroll
-        for (int q = 0; q < kTokens; q += 4) {
+        for (int q = 0; q < kTokens / 4; ++q) {
           if constexpr (share_size<8, NL>() == 2)
-            *reinterpret_cast<float2*>(&s.ys[buf][q + at / 2][lc]) = make_float2(v[q / 4][0], v[q / 4][1]);
+            *reinterpret_cast<float2*>(&s.ys[buf][4 * q + at / 2][lc]) = make_float2(v[q][0], v[q][1]);
           else if (nl < share_lanes<8, NL>())
-            s.ys[buf][q + at / 2][lc + at % 2] = v[q / 4][0];
+            s.ys[buf][4 * q + at / 2][lc + at % 2] = v[q][0];
         }
       }
       // The element-wise half waits for every tile forward, for those whose buffer it fills again otherwise.
