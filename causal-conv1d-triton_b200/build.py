@@ -148,7 +148,7 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     for inc in ce.include_paths() + [cuda_inc, sysconfig.get_paths()["include"], INCLUDE]:
         flags += ["-I", inc]
     link = [cxx, "-shared"] + objs + ["-L", os.path.dirname(LIB), "-lcausal_conv1d_b200", "-L", torch_lib, "-lc10",
-                                      "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN",
+                                      "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN",
                                       f"-Wl,-rpath,{torch_lib}", "-o", TORCH_EXT]
 
     def run(cmd):

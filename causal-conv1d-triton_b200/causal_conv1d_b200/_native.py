@@ -140,6 +140,9 @@ class CausalConv1dError(RuntimeError):
     """A non-zero status returned by the C ABI."""
 
 
+tex.set_error_class(CausalConv1dError)
+
+
 def check(code: int, what: str) -> None:
     if code != CC1D_OK:
         msg = lib.cc1d_error_string(code).decode()

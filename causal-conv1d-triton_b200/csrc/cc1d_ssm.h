@@ -68,7 +68,7 @@ struct SsmUpdateParams {
   void* out;               // (batch, seqlen, dim) contiguous
   int batch, seqlen, dim, dstate, group_dim;
   int softplus;
-  int blocks, state_vec;   // set by the launcher: CTAs over the channels; 4 states are one aligned vector
+  int blocks;              // set by the launcher: CTAs over the channels
 };
 
 int record_cuda_error(cudaError_t e);  // sets cc1d_last_cuda_error(), returns CC1D_ERR_CUDA

@@ -58,7 +58,22 @@ int plan_for(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t
   int sms = 0;
   const int rc = device_sms(&sms);
   if (rc != CC1D_OK) return rc;
-  *plan = make_plan(batch, seqlen, dim, dstate, groups, backward, sms);
+  // The last few plans of the thread: a layer asks for the same ones again, twice a call.
+  struct Known {
+    int64_t key[6];
+    Plan plan;
+  };
+  thread_local Known known[8] = {};
+  thread_local unsigned next = 0;
+  const int64_t key[6] = {batch, seqlen, dim, dstate, 2 * groups + (backward ? 1 : 0), sms};
+  bool found = false;
+  for (const Known& k : known)
+    if (k.plan.segs > 0 && std::equal(key, key + 6, k.key)) *plan = k.plan, found = true;
+  if (!found) {
+    *plan = make_plan(batch, seqlen, dim, dstate, groups, backward, sms);
+    Known& k = known[next++ % 8];
+    std::copy(key, key + 6, k.key), k.plan = *plan;
+  }
   if (batch * plan->segs * groups * plan->blocks > kMaxInt) return CC1D_ERR_INVALID;
   return CC1D_OK;
 }

@@ -481,7 +481,7 @@ template <typename T, int NL, bool SEQ>
 cudaError_t launch_main(const SsmParams& p, cudaStream_t s) {
   constexpr int smem = static_cast<int>(sizeof(BwdSmem<T, NL>));
   const auto kernel = cc1d_ssm_bwd_kernel<T, NL, SEQ>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = allow_smem<cc1d_ssm_bwd_kernel<T, NL, SEQ>>(smem);
   if (e != cudaSuccess) return e;
   // setmaxnreg would wait for registers that a launch with fewer of them does not have.
   static const bool holds_split = [&] {

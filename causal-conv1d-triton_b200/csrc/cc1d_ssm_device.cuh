@@ -2,6 +2,8 @@
 // vectors of 8 channels, and sums across lanes that leave each lane with its own share.
 #pragma once
 
+#include <atomic>
+
 #include "cc1d_device.cuh"
 #include "cc1d_ssm.h"
 
@@ -243,6 +245,21 @@ constexpr int share_lanes() {
     return 2 * share_lanes<V / 2, L / 2>();
   else
     return 1;
+}
+
+// Raises a kernel's dynamic shared memory limit, once per device and kernel (one flag per template
+// instance of the caller). Repeating it would be harmless; it costs a microsecond.
+template <auto KERNEL>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (ready.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 // A CTA's two halves, a walk and the element-wise work around it, hand tiles to each other in

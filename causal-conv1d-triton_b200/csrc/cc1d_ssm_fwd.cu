@@ -364,10 +364,9 @@ __global__ void __launch_bounds__(128) cc1d_ssm_join_kernel(const float* __restr
 template <typename T, int NL, int PASS, bool SEQ>
 cudaError_t launch(const SsmParams& p, cudaStream_t s) {
   constexpr int smem = static_cast<int>(sizeof(ScanSmem<T, NL>));
-  const auto kernel = cc1d_ssm_scan_kernel<T, NL, PASS, SEQ>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = allow_smem<cc1d_ssm_scan_kernel<T, NL, PASS, SEQ>>(smem);
   if (e != cudaSuccess) return e;
-  kernel<<<static_cast<unsigned>(p.batch) * p.segs * p.groups * p.blocks, kThreads, smem, s>>>(p);
+  cc1d_ssm_scan_kernel<T, NL, PASS, SEQ><<<static_cast<unsigned>(p.batch) * p.segs * p.groups * p.blocks, kThreads, smem, s>>>(p);
   return cudaGetLastError();
 }
 

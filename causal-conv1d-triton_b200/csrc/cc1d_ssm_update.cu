@@ -17,48 +17,56 @@ namespace {
 
 constexpr int kRows = 4;
 
-template <typename T, typename ST, int NL>
-__global__ void __launch_bounds__(256, 3) cc1d_ssm_update_kernel(const __grid_constant__ SsmUpdateParams p) {
+// 4 consecutive elements of a buffer whose type is given at run time, the first `n` of them.
+__device__ __forceinline__ void ld_any4(const void* base, int64_t i, int dtype, int n, float (&v)[4]) {
+#pragma unroll
+  for (int m = 0; m < 4; ++m) v[m] = 0.0f;
+  if (dtype == kF32) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      if (m < n) v[m] = static_cast<const float*>(base)[i + m];
+  } else {
+    for (int m = 0; m < n && m < 4; ++m) v[m] = ld_any(base, i + m, dtype);
+  }
+}
+
+// VEC: a lane's 4 states are one aligned vector, and so are its B and C. Without it they move one by one.
+template <typename T, typename ST, int NL, bool VEC>
+__global__ void __launch_bounds__(256, VEC ? 4 : 2) cc1d_ssm_update_kernel(const __grid_constant__ SsmUpdateParams p) {
   const int nl = threadIdx.x % NL, n0 = 4 * nl;
   const int ch = static_cast<int>(blockIdx.x % p.blocks) * (256 / NL) + static_cast<int>(threadIdx.x) / NL;
   const int b0 = static_cast<int>(blockIdx.x / p.blocks) * kRows;
-  const bool in = ch < p.dim;
-  const int g = in ? ch / p.group_dim : 0;
-  const int nn = in ? p.dstate - n0 : 0;  // states of this lane
-  const bool whole = p.state_vec && nn >= 4;
+  const int nn = ch < p.dim ? p.dstate - n0 : 0;  // states of this lane
 
-  // Slots of the rows; a negative one (or one past the end) marks a padded entry: nothing of it is
-  // read or written.
-  int64_t at[kRows];
-  bool live[kRows];
+  // The rows' states; null for a padded entry (a negative slot, or one past the end), of which nothing
+  // is read or written.
+  ST* st[kRows];
   float2 h[kRows][2];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int b = b0 + r;
     const int64_t slot = b >= p.batch ? -1 : (p.indices != nullptr ? p.indices[b] : b);
-    live[r] = in && slot >= 0 && slot < p.slots;
-    at[r] = (slot * p.dim + ch) * p.dstate + n0;
+    const bool live = ch < p.dim && slot >= 0 && slot < p.slots;
+    st[r] = live ? static_cast<ST*>(p.state) + (slot * p.dim + ch) * p.dstate + n0 : nullptr;
   }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    const ST* st = static_cast<const ST*>(p.state) + at[r];
     h[r][0] = h[r][1] = make_float2(0.f, 0.f);
-    if (live[r]) {
-      if (whole) {
-        load_vec<ST, 4>(st, h[r]);
+    if (st[r] != nullptr) {
+      if (VEC) {
+        if (nn > 0) load_vec<ST, 4>(st[r], h[r]);
       } else {
-        if (nn > 0) h[r][0].x = to_f<ST>(st[0]);
-        if (nn > 1) h[r][0].y = to_f<ST>(st[1]);
-        if (nn > 2) h[r][1].x = to_f<ST>(st[2]);
-        if (nn > 3) h[r][1].y = to_f<ST>(st[3]);
+        if (nn > 0) h[r][0].x = to_f<ST>(st[r][0]);
+        if (nn > 1) h[r][0].y = to_f<ST>(st[r][1]);
+        if (nn > 2) h[r][1].x = to_f<ST>(st[r][2]);
+        if (nn > 3) h[r][1].y = to_f<ST>(st[r][3]);
       }
     }
   }
+  const bool in = ch < p.dim;
   float a[4];
-#pragma unroll
-  for (int m = 0; m < 4; ++m)
-    a[m] = m < nn ? ld_any(p.A.ptr, static_cast<int64_t>(ch) * p.dstate + n0 + m, p.A.dtype) * kLog2e : 0.0f;
-  const float2 A2[2] = {make_float2(a[0], a[1]), make_float2(a[2], a[3])};
+  ld_any4(p.A.ptr, static_cast<int64_t>(ch) * p.dstate + n0, p.A.dtype, nn, a);
+  const float2 A2[2] = {make_float2(a[0] * kLog2e, a[1] * kLog2e), make_float2(a[2] * kLog2e, a[3] * kLog2e)};
   const float skip = in && p.D.ptr != nullptr ? ld_any(p.D.ptr, ch, p.D.dtype) : 0.0f;
   const float bias = in && p.dt_bias.ptr != nullptr ? ld_any(p.dt_bias.ptr, ch, p.dt_bias.dtype) : 0.0f;
 
@@ -66,11 +74,13 @@ __global__ void __launch_bounds__(256, 3) cc1d_ssm_update_kernel(const __grid_co
   const int own = lane_share<kRows, NL, 1>(), ob = b0 + own;
   bool own_live = false;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) own_live = r == own ? live[r] : own_live;
+  for (int r = 0; r < kRows; ++r) own_live = r == own ? st[r] != nullptr : own_live;
   const int lead = threadIdx.x & 31 & ~(NL - 1);  // the channel's first lane
+  const int g = in ? ch / p.group_dim : 0;
   const T* bp = static_cast<const T*>(p.Bm.ptr) + g * p.Bm.sg;
   const T* cp = static_cast<const T*>(p.Cm.ptr) + g * p.Cm.sg;
 
+#pragma unroll 1
   for (int64_t l = 0; l < p.seqlen; ++l) {
     float x = 0.0f, delta = 0.0f, z = 0.0f;
     if (own_live) {
@@ -78,13 +88,13 @@ __global__ void __launch_bounds__(256, 3) cc1d_ssm_update_kernel(const __grid_co
       delta = to_f<T>(static_cast<const T*>(p.dt.ptr)[ob * p.dt.sb + l * p.dt.st + ch]) + bias;
       if (p.z.ptr != nullptr) z = to_f<T>(static_cast<const T*>(p.z.ptr)[ob * p.z.sb + l * p.z.st + ch]);
     }
-    Raw4<T> rB[kRows], rC[kRows];
+    Raw4<T> B[kRows], C[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      rB[r] = rC[r] = zero4<T>();
-      if (live[r] && nn > 0) {
-        rB[r] = load4(bp + (b0 + r) * p.Bm.sb + l * p.Bm.st, n0, p.dstate, p.Bm.vec);
-        rC[r] = load4(cp + (b0 + r) * p.Cm.sb + l * p.Cm.st, n0, p.dstate, p.Cm.vec);
+      B[r] = C[r] = zero4<T>();
+      if (st[r] != nullptr && nn > 0) {
+        B[r] = load4(bp + (b0 + r) * p.Bm.sb + l * p.Bm.st, n0, VEC ? kSsmMaxState : p.dstate, VEC);
+        C[r] = load4(cp + (b0 + r) * p.Cm.sb + l * p.Cm.st, n0, VEC ? kSsmMaxState : p.dstate, VEC);
       }
     }
     if (p.softplus) delta = softplus(delta);
@@ -95,11 +105,11 @@ __global__ void __launch_bounds__(256, 3) cc1d_ssm_update_kernel(const __grid_co
       // The lane with share r: bits 0 and 1 of its place hold the halves in that order.
       const int from = lead + ((r >> 1) | ((r & 1) << 1));
       const float2 d = splat(__shfl_sync(0xffffffffu, delta, from)), v = splat(__shfl_sync(0xffffffffu, u, from));
-      const float4 B = unpack4(rB[r]), C = unpack4(rC[r]);
+      const float4 b = unpack4(B[r]), c = unpack4(C[r]);
       const float2 a0 = exp2_approx2(fmul2(d, A2[0])), a1 = exp2_approx2(fmul2(d, A2[1]));
-      h[r][0] = ffma2(a0, h[r][0], fmul2(v, make_float2(B.x, B.y)));
-      h[r][1] = ffma2(a1, h[r][1], fmul2(v, make_float2(B.z, B.w)));
-      const float2 s = ffma2(h[r][1], make_float2(C.z, C.w), fmul2(h[r][0], make_float2(C.x, C.y)));
+      h[r][0] = ffma2(a0, h[r][0], fmul2(v, make_float2(b.x, b.y)));
+      h[r][1] = ffma2(a1, h[r][1], fmul2(v, make_float2(b.z, b.w)));
+      const float2 s = ffma2(h[r][1], make_float2(c.z, c.w), fmul2(h[r][0], make_float2(c.x, c.y)));
       y[r] = s.x + s.y;
     }
     lane_sums<kRows, NL, 1>(y);
@@ -111,32 +121,39 @@ __global__ void __launch_bounds__(256, 3) cc1d_ssm_update_kernel(const __grid_co
   }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    ST* st = static_cast<ST*>(p.state) + at[r];
-    if (live[r]) {
-      if (whole) {
-        store_vec<ST, 4>(st, h[r]);
+    if (st[r] != nullptr) {
+      if (VEC) {
+        if (nn > 0) store_vec<ST, 4>(st[r], h[r]);
       } else {
-        if (nn > 0) st[0] = from_f<ST>(h[r][0].x);
-        if (nn > 1) st[1] = from_f<ST>(h[r][0].y);
-        if (nn > 2) st[2] = from_f<ST>(h[r][1].x);
-        if (nn > 3) st[3] = from_f<ST>(h[r][1].y);
+        if (nn > 0) st[r][0] = from_f<ST>(h[r][0].x);
+        if (nn > 1) st[r][1] = from_f<ST>(h[r][0].y);
+        if (nn > 2) st[r][2] = from_f<ST>(h[r][1].x);
+        if (nn > 3) st[r][3] = from_f<ST>(h[r][1].y);
       }
     }
   }
+}
+
+template <typename T, typename ST, int NL>
+void launch(const SsmUpdateParams& p, bool vec, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>(p.blocks) * ((p.batch + kRows - 1) / kRows);
+  if (vec)
+    cc1d_ssm_update_kernel<T, ST, NL, true><<<grid, 256, 0, s>>>(p);
+  else
+    cc1d_ssm_update_kernel<T, ST, NL, false><<<grid, 256, 0, s>>>(p);
 }
 
 template <typename T, typename ST>
 cudaError_t launch(SsmUpdateParams p, cudaStream_t s) {
   const int nl = ssm_lanes(p.dstate);
   p.blocks = static_cast<int>((static_cast<int64_t>(p.dim) * nl + 255) / 256);
-  p.state_vec = p.dstate % 4 == 0 && reinterpret_cast<uintptr_t>(p.state) % (4 * sizeof(ST)) == 0;
-  const unsigned grid = static_cast<unsigned>(p.blocks) * ((p.batch + kRows - 1) / kRows);
+  const bool vec = p.dstate % 4 == 0 && reinterpret_cast<uintptr_t>(p.state) % (4 * sizeof(ST)) == 0 && p.Bm.vec && p.Cm.vec;
   if (nl == 4)
-    cc1d_ssm_update_kernel<T, ST, 4><<<grid, 256, 0, s>>>(p);
+    launch<T, ST, 4>(p, vec, s);
   else if (nl == 8)
-    cc1d_ssm_update_kernel<T, ST, 8><<<grid, 256, 0, s>>>(p);
+    launch<T, ST, 8>(p, vec, s);
   else
-    cc1d_ssm_update_kernel<T, ST, 16><<<grid, 256, 0, s>>>(p);
+    launch<T, ST, 16>(p, vec, s);
   return cudaGetLastError();
 }
 
