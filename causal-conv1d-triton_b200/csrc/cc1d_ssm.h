@@ -45,6 +45,7 @@ struct SsmParams {
   // Sequences in pieces, (batch, segs, dim, 4 NL) each: the state (gradient) that a piece leaves when it
   // receives none, its decay, and what it receives.
   float *seg_out, *seg_decay, *seg_in;
+  int fold;  // no join kernel ran: each piece works out what it receives
   // Backward
   SsmTokens dout;
   SsmParam dfinal;             // (batch, dim, dstate) or null

@@ -21,6 +21,11 @@ int elem_size(int dtype) { return dtype == kF32 ? 4 : 2; }
 bool valid_dtype(int dtype) { return dtype == kF32 || dtype == kF16 || dtype == kBF16; }
 bool valid_param(const cc1d_param& q) { return q.ptr == nullptr || valid_dtype(q.dtype); }
 
+// Up to this many pieces each piece works out what it receives from the ones before it, which spares a
+// launch; the work grows with the square of their number, so above it the join kernel does it once
+// (1 x 512 x 512 channels in 16 pieces: %s).
+constexpr int kFoldSegs = 16;
+
 // How one direction runs: CTAs that cover a group's channels, pieces of the sequence and their length.
 struct Plan {
   int nl, blocks, segs, seg_len;
@@ -129,6 +134,7 @@ SsmParams common(const cc1d_ssm_problem& q, const Plan& plan) {
 }
 
 void set_pieces(SsmParams& p, float* ws, int64_t floats) {
+  p.fold = p.segs <= kFoldSegs;
   p.seg_out = ws, p.seg_decay = ws + floats / 3, p.seg_in = ws + 2 * (floats / 3);
 }
 
@@ -181,7 +187,7 @@ int cc1d_ssm_fwd(const cc1d_ssm_problem* q, void* out, float* final_states, floa
   if (plan.segs > 1) {
     set_pieces(p, static_cast<float*>(workspace), need);
     CC1D_TRY(done(launch_ssm_scan(p, kSsmPieceForward, q->x_dtype, s)));
-    CC1D_TRY(done(launch_ssm_join(p, false, s)));
+    if (!p.fold) CC1D_TRY(done(launch_ssm_join(p, false, s)));
   }
   return done(launch_ssm_scan(p, kSsmForward, q->x_dtype, s));
 }
@@ -216,7 +222,7 @@ int cc1d_ssm_bwd(const cc1d_ssm_problem* q, const cc1d_tokens* dout, const float
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (plan.segs > 1) {
     CC1D_TRY(done(launch_ssm_scan(p, kSsmPieceBackward, q->x_dtype, s)));
-    CC1D_TRY(done(launch_ssm_join(p, true, s)));
+    if (!p.fold) CC1D_TRY(done(launch_ssm_join(p, true, s)));
   }
   return done(launch_ssm_bwd(p, q->x_dtype, s));
 }

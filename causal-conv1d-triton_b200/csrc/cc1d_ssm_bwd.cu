@@ -99,9 +99,19 @@ struct Bwd {
     };
     fetch(0, 0);
 
-    float sums[2][8];  // dD and ddt_bias of the thread's channels
+    // dB and dC of the CTA: element tid + k * 128 of a tile's rows of 2 NP.
+    constexpr int SUMS = kTokens * 2 * NP / kSsmHalf, ROWS = kSsmHalf / (2 * NP);  // per thread; rows between two of them
+    static_assert(kSsmHalf % (2 * NP) == 0 && SUMS * kSsmHalf == kTokens * 2 * NP, "");
+    const int br = tid / (2 * NP), bk = tid % (2 * NP);
+    const int64_t bc_row = static_cast<int64_t>(p.groups) * p.blocks * (2 * NP);
+    float* const part_bc = p.part_bc + (static_cast<int64_t>(w.b) * p.seqlen + br) * bc_row + (w.g * p.blocks + w.blk) * (2 * NP) + bk;
+    const bool out_vec = (p.dim * sizeof(T)) % 16 == 0 && (w.c0 * sizeof(T)) % 16 == 0;
+    const int64_t out = (static_cast<int64_t>(w.b) * p.seqlen + er) * p.dim + w.c0 + ec;
+    const int turn = ec >> 4 & 3;
+
+    float2 sums[2][4];  // dD and ddt_bias of the thread's channels
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sums[0][i] = sums[1][i] = 0.0f;
+    for (int i = 0; i < 4; ++i) sums[0][i] = sums[1][i] = make_float2(0.f, 0.f);
     uint32_t off0 = 0, off1 = 0, off2 = 0;
     int ring = 0;
     for (int it = 0; it < tiles + 2; ++it, ring = next_stage(ring)) {
@@ -111,46 +121,51 @@ struct Bwd {
         const int t = w.t0 + (tiles + 1 - it) * kTokens, old = next_stage(ring);  // two tiles ago
         take_over(done_barrier(buf));
         if (work && t + er < w.t1) {
-          const bool off = SEQ && ((off2 >> er) & 1u);
-          const int64_t at = (static_cast<int64_t>(w.b) * p.seqlen + t + er) * p.dim + w.c0 + ec;
-          const bool out_vec = (p.dim * sizeof(T)) % 16 == 0 && (w.c0 * sizeof(T)) % 16 == 0;
-          float x[8], o[8], v[8];
-          unpack8(read8<T>(&s.raw[old][0][0][tid], kSsmHalf), x);
-          unpack8(read8<T>(&s.raw[old][3][0][tid], kSsmHalf), o);
-          if (has_z) {
-            float z[8];
-            unpack8(read8<T>(&s.raw[old][2][0][tid], kSsmHalf), z);
+          const int64_t at = out + static_cast<int64_t>(t) * p.dim;
+          float2 dx[4], dd[4], dz[4];
+          if (SEQ && ((off2 >> er) & 1u)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float sg = sigmoid(z[i]), yt = fmaf(s.sk[0][ec + i], x[i], s.f[buf][0][er][ec + i]);
-              v[i] = off ? 0.0f : o[i] * yt * sg * fmaf(z[i], 1.0f - sg, 1.0f);  // dz
-              o[i] *= z[i] * sg;                                                  // dy
+            for (int i = 0; i < 4; ++i) dx[i] = dd[i] = dz[i] = make_float2(0.f, 0.f);
+          } else {
+            float2 x[4], o[4], v[4], skip[4];
+            unpack8(read8<T>(&s.raw[old][0][0][tid], kSsmHalf), x);
+            unpack8(read8<T>(&s.raw[old][3][0][tid], kSsmHalf), o);
+            pairs8(&s.sk[0][ec], skip);
+            if (has_z) {
+              float2 z[4];
+              unpack8(read8<T>(&s.raw[old][2][0][tid], kSsmHalf), z);
+              pairs8(&s.f[buf][0][er][ec], v);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 sg = sigmoid2(z[i]), y = ffma2(skip[i], x[i], v[i]);
+                const float2 rest = make_float2(1.0f - sg.x, 1.0f - sg.y);  // silu' = sg (1 + z (1 - sg))
+                dz[i] = fmul2(fmul2(o[i], y), fmul2(sg, ffma2(z[i], rest, splat(1.0f))));
+                o[i] = fmul2(o[i], fmul2(z[i], sg));  // dy
+              }
             }
-            store8(static_cast<T*>(p.dz) + at, v, en, out_vec);
-          }
-          float dx[8], d[8];
-          unpack8(read8<T>(&s.raw[old][1][0][tid], kSsmHalf), d);
+            float2 gb[4], qa[4], bias[4];
+            unpack8(read8<T>(&s.raw[old][1][0][tid], kSsmHalf), v);
+            pairs8(&s.f[buf][1][er][ec], gb), pairs8(&s.f[buf][2][er][ec], qa), pairs8(&s.sk[1][ec], bias);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float gb = s.f[buf][1][er][ec + i], qa = s.f[buf][2][er][ec + i];
-            const float4 du = s.du[buf][er][(ec >> 1) + ((i >> 1) ^ (ec >> 4 & 3))];
-            const float delta = i % 2 ? du.y : du.x;
-            const float slope = p.softplus ? sigmoid(d[i] + s.sk[1][ec + i]) : 1.0f;
-            v[i] = off ? 0.0f : slope * fmaf(x[i], gb, kLn2 * qa);
-            dx[i] = off ? 0.0f : fmaf(delta, gb, s.sk[0][ec + i] * o[i]);
-            sums[0][i] += off ? 0.0f : o[i] * x[i];
-            sums[1][i] += v[i];
+            for (int i = 0; i < 4; ++i) {
+              const float2 delta = *reinterpret_cast<const float2*>(&s.du[buf][er][(ec >> 1) + (i ^ turn)]);
+              dd[i] = ffma2(x[i], gb[i], fmul2(qa[i], splat(kLn2)));
+              if (p.softplus) dd[i] = fmul2(dd[i], sigmoid2(fadd2(v[i], bias[i])));
+              dx[i] = ffma2(delta, gb[i], fmul2(skip[i], o[i]));
+              sums[0][i] = ffma2(o[i], x[i], sums[0][i]);
+              sums[1][i] = fadd2(sums[1][i], dd[i]);
+            }
           }
+          if (has_z) store8(static_cast<T*>(p.dz) + at, dz, en, out_vec);
           store8(static_cast<T*>(p.dx) + at, dx, en, out_vec);
-          store8(static_cast<T*>(p.ddt) + at, v, en, out_vec);
+          store8(static_cast<T*>(p.ddt) + at, dd, en, out_vec);
         }
-        const int64_t tok = static_cast<int64_t>(w.b) * p.seqlen + t;
-        for (int i = tid; i < kTokens * 2 * NP; i += kSsmHalf) {
-          const int r = i / (2 * NP), k = i % (2 * NP);
-          if (t + r < w.t1) {
-            const float v = (s.dbc[buf][0][r][k] + s.dbc[buf][1][r][k]) + (s.dbc[buf][2][r][k] + s.dbc[buf][3][r][k]);
-            p.part_bc[(((tok + r) * p.groups + w.g) * p.blocks + w.blk) * (2 * NP) + k] = v;
-          }
+        const float* d = &s.dbc[buf][0][br][bk];
+#pragma unroll
+        for (int k = 0; k < SUMS; ++k, d += ROWS * 2 * NP) {
+          constexpr int W = kTokens * 2 * NP;  // from one warp's to the next one's
+          const float v = (d[0] + d[W]) + (d[2 * W] + d[3 * W]);
+          if (t + br + k * ROWS < w.t1) part_bc[(t + k * ROWS) * bc_row] = v;
         }
       }
       if (it < tiles) {
@@ -160,30 +175,33 @@ struct Bwd {
         if (SEQ) seq = seq_bits(*ids[buf], p, t);
         off0 = seq.pad;
         if (er < kTokens) {
-          float x[8], d[8], o[8];
-          unpack8(read8<T>(&s.raw[ring][0][0][tid], kSsmHalf), x);
-          unpack8(read8<T>(&s.raw[ring][1][0][tid], kSsmHalf), d);
-          unpack8(read8<T>(&s.raw[ring][3][0][tid], kSsmHalf), o);
+          float4* const dst = &s.du[buf][er][ec >> 1];  // a pair's place within its vector is turned as in the forward
+          float4* const dy = reinterpret_cast<float4*>(&s.f[buf][0][er][ec]);
           // Padding takes no step and has no input; neither has what lies outside the piece.
-          const bool in = work && t + er < w.t1 && !(SEQ && ((seq.pad >> er) & 1u));
-          if (has_z) {
-            float z[8];
-            unpack8(read8<T>(&s.raw[ring][2][0][tid], kSsmHalf), z);
+          if (work && t + er < w.t1 && !(SEQ && ((seq.pad >> er) & 1u))) {
+            float2 x[4], d[4], o[4], bias[4];
+            unpack8(read8<T>(&s.raw[ring][0][0][tid], kSsmHalf), x);
+            unpack8(read8<T>(&s.raw[ring][1][0][tid], kSsmHalf), d);
+            unpack8(read8<T>(&s.raw[ring][3][0][tid], kSsmHalf), o);
+            pairs8(&s.sk[1][ec], bias);
+            if (has_z) {
+              float2 z[4];
+              unpack8(read8<T>(&s.raw[ring][2][0][tid], kSsmHalf), z);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] *= z[i] * sigmoid(z[i]);
-          }
+              for (int i = 0; i < 4; ++i) o[i] = fmul2(o[i], fmul2(z[i], sigmoid2(z[i])));
+            }
+            dy[0] = make_float4(o[0].x, o[0].y, o[1].x, o[1].y), dy[1] = make_float4(o[2].x, o[2].y, o[3].x, o[3].y);
 #pragma unroll
-          for (int i = 0; i < 8; i += 4)
-            *reinterpret_cast<float4*>(&s.f[buf][0][er][ec + i]) =
-                in ? make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < 4; ++i) {
+              float2 delta = fadd2(d[i], bias[i]);
+              if (p.softplus) delta = softplus2(delta);
+              const float2 u = fmul2(delta, x[i]);
+              dst[i ^ turn] = make_float4(delta.x, delta.y, u.x, u.y);
+            }
+          } else {
+            dy[0] = dy[1] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float2 delta = fadd2(make_float2(d[2 * i], d[2 * i + 1]), make_float2(s.sk[1][ec + 2 * i], s.sk[1][ec + 2 * i + 1]));
-            if (p.softplus) delta = softplus2(delta);
-            const float2 u = fmul2(delta, make_float2(x[2 * i], x[2 * i + 1]));
-            // A pair's place within its vector is turned as in the forward.
-            s.du[buf][er][(ec >> 1) + (i ^ (ec >> 4 & 3))] =
-                in ? make_float4(delta.x, delta.y, u.x, u.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < 4; ++i) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
 #pragma unroll
@@ -208,7 +226,7 @@ struct Bwd {
     for (int k = 0; k < 2; ++k) {
       named_sync(7, kSsmHalf);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) col[i * kSsmHalf + tid] = sums[k][i];
+      for (int i = 0; i < 8; ++i) col[i * kSsmHalf + tid] = i % 2 ? sums[k][i / 2].y : sums[k][i / 2].x;
       named_sync(7, kSsmHalf);
       for (int c = tid; c < w.nc; c += kSsmHalf) {
         float v = 0.0f;
@@ -382,12 +400,15 @@ struct Bwd {
         v[m] = 0.0f;
         if (in && last && p.dfinal.ptr != nullptr)
           v[m] = ld_any(p.dfinal.ptr, (static_cast<int64_t>(w.b) * p.dim + ch) * p.dstate + n, p.dfinal.dtype);
-        if (in && !last) v[m] = p.seg_in[(row_bs * p.dim + ch) * NP + n];
       }
       A2[c][0] = make_float2(a[0], a[1]), A2[c][1] = make_float2(a[2], a[3]);
       g[c][0] = make_float2(v[0], v[1]), g[c][1] = make_float2(v[2], v[3]);
       dA[c][0] = dA[c][1] = make_float2(0.f, 0.f);
     }
+    if (!last) piece_in(p, w, NP, w.c0 + lc, n1, n2, true, g);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      if (lc + c >= w.nc) g[c][0] = g[c][1] = make_float2(0.f, 0.f);  // no channel: nothing for the sums over channels
 
 #pragma unroll 1
     for (int it = 0; it < tiles; ++it) {
@@ -452,6 +473,7 @@ __global__ void __launch_bounds__(256) cc1d_ssm_finish_kernel(const __grid_const
     const int64_t row = i / (2 * p.dstate);  // token and group
     const float* src = p.part_bc + row * p.blocks * (2 * np) + which * np + n;
     float v = 0.0f;
+#pragma unroll 8
     for (int q = 0; q < p.blocks; ++q) v += src[static_cast<int64_t>(q) * 2 * np];
     static_cast<T*>(which ? p.dC : p.dB)[row * p.dstate + n] = from_f<T>(v);
     return;
@@ -461,7 +483,7 @@ __global__ void __launch_bounds__(256) cc1d_ssm_finish_kernel(const __grid_const
   if (i < n_a) {
     const float* src = p.part_a + i / p.dstate * np + i % p.dstate;
     float v = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
     for (int q = 0; q < rows; ++q) v += src[static_cast<int64_t>(q) * p.dim * np];
     st_any(p.dA, i, p.A.dtype, v);
     return;
@@ -470,7 +492,7 @@ __global__ void __launch_bounds__(256) cc1d_ssm_finish_kernel(const __grid_const
   if (i < 2ll * p.dim) {
     const int k = static_cast<int>(i / p.dim), ch = static_cast<int>(i % p.dim);
     float v = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
     for (int q = 0; q < rows; ++q) v += p.part_d[(static_cast<int64_t>(q) * 2 + k) * p.dim + ch];
     if (k == 0 && p.dD != nullptr) st_any(p.dD, ch, p.D.dtype, v);
     if (k == 1 && p.ddt_bias != nullptr) st_any(p.ddt_bias, ch, p.dt_bias.dtype, v);

@@ -26,7 +26,7 @@ __device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
 // at most (s = 1/3) and keeps its relative accuracy as w goes to 0, where the step size is small.
 // A NaN comes through s.
 __device__ __forceinline__ float2 softplus2(float2 v) {
-  const float2 w = make_float2(__expf(-fabsf(v.x)), __expf(-fabsf(v.y)));
+  const float2 w = exp2_approx2(fmul2(make_float2(fabsf(v.x), fabsf(v.y)), splat(-kLog2e)));
   const float2 s = make_float2(__fdividef(w.x, 2.0f + w.x), __fdividef(w.y, 2.0f + w.y)), q = fmul2(s, s);
   float2 r = ffma2(q, splat(1.0f / 13), splat(1.0f / 11));
   r = ffma2(r, q, splat(1.0f / 9));
@@ -38,7 +38,11 @@ __device__ __forceinline__ float2 softplus2(float2 v) {
 }
 __device__ __forceinline__ float softplus(float v) { return softplus2(splat(v)).x; }
 
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+__device__ __forceinline__ float2 sigmoid2(float2 v) {
+  const float2 w = exp2_approx2(fmul2(v, splat(-kLog2e))), d = fadd2(w, splat(1.0f));
+  return make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+}
+__device__ __forceinline__ float sigmoid(float v) { return sigmoid2(splat(v)).x; }
 
 // 8 channels of one token as loaded, before conversion: a thread keeps the next tile's in registers.
 template <typename T>
@@ -80,35 +84,40 @@ __device__ __forceinline__ Raw8<T> zero8() {
 }
 
 template <typename T>
-__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float2 (&v)[4]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.w[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = word_to_f2<T>(r.w[i]);
-      v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    }
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) v[i] = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+    else v[i] = word_to_f2<T>(r.w[i]);
   }
 }
 
 // Rounds and stores channels [0, n) of 8.
 template <typename T>
-__device__ __forceinline__ void store8(T* dst, const float (&v)[8], int n, bool vec) {
+__device__ __forceinline__ void store8(T* dst, const float2 (&v)[4], int n, bool vec) {
   if (vec && n == 8) {
+    constexpr int C = 16 / static_cast<int>(sizeof(T));
 #pragma unroll
-    for (int i = 0; i < 8; i += 16 / static_cast<int>(sizeof(T))) {
-      constexpr int C = 16 / static_cast<int>(sizeof(T));
+    for (int i = 0; i < 8; i += C) {
       float2 f[C / 2];
 #pragma unroll
-      for (int k = 0; k < C / 2; ++k) f[k] = make_float2(v[i + 2 * k], v[i + 2 * k + 1]);
+      for (int k = 0; k < C / 2; ++k) f[k] = v[i / 2 + k];
       store_vec<T, C>(dst + i, f);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) dst[i] = from_f<T>(v[i]);
+    for (int i = 0; i < 4; ++i) {
+      if (2 * i < n) dst[2 * i] = from_f<T>(v[i].x);
+      if (2 * i + 1 < n) dst[2 * i + 1] = from_f<T>(v[i].y);
+    }
+  }
+}
+// 8 consecutive floats of shared memory at a multiple of 8.
+__device__ __forceinline__ void pairs8(const float* src, float2 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float4 q = reinterpret_cast<const float4*>(src)[i];
+    v[2 * i] = make_float2(q.x, q.y), v[2 * i + 1] = make_float2(q.z, q.w);
   }
 }
 
@@ -293,6 +302,42 @@ __device__ __forceinline__ SsmPlace ssm_place(const SsmParams& p) {
   w.t0 = w.seg * p.seg_len;
   w.t1 = min(p.seqlen, w.t0 + p.seg_len);
   return w;
+}
+
+// What piece w.seg of the sequence receives, into h: of channels ch and ch + 1 the pairs of states that
+// start at n1 and n2. From the join kernel, or, with few pieces, by the same chain over the pieces before
+// (after) it, whose loads are independent of it.
+__device__ __forceinline__ void piece_in(const SsmParams& p, const SsmPlace& w, int np, int ch, int n1, int n2, bool backward,
+                                         float2 (&h)[2][2]) {
+  const int64_t row = static_cast<int64_t>(p.dim) * np;
+  int64_t at[2][2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    // A channel past the last one reads the last one's.
+    const int64_t q = w.b * p.segs * row + static_cast<int64_t>(min(ch + c, p.dim - 1)) * np;
+    at[c][0] = q + n1, at[c][1] = q + n2;
+  }
+  auto read = [&](const float* base, int seg, float2 (&v)[2][2]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) v[c][m] = *reinterpret_cast<const float2*>(base + at[c][m] + seg * row);
+  };
+  if (!p.fold) return read(p.seg_in, w.seg, h);
+  const int from = backward ? p.segs - 1 : 0, step = backward ? -1 : 1, n = backward ? p.segs - 1 - w.seg : w.seg;
+  read(p.seg_out, from, h);
+#pragma unroll 4
+  for (int i = 1; i < n; ++i) {
+    float2 o[2][2], d[2][2];
+    read(p.seg_out, from + i * step, o), read(p.seg_decay, from + i * step, d);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        h[c][m].x = d[c][m].x == 0.0f ? o[c][m].x : fmaf(d[c][m].x, h[c][m].x, o[c][m].x);
+        h[c][m].y = d[c][m].y == 0.0f ? o[c][m].y : fmaf(d[c][m].y, h[c][m].y, o[c][m].y);
+      }
+  }
 }
 
 // Tokens of a tile (bit i: token t + i of row b) whose state starts from zero because the sequence id

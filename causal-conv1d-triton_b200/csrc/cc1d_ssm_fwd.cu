@@ -68,12 +68,16 @@ struct Scan {
     const T* bp = static_cast<const T*>(p.Bm.ptr) + w.b * p.Bm.sb + w.g * p.Bm.sg;
     const T* cp = static_cast<const T*>(p.Cm.ptr) + w.b * p.Cm.sb + w.g * p.Cm.sg;
     const bool has_z = PASS != kSsmPieceForward && p.z.ptr != nullptr;
-    float skip[8], bias[8];
+    float2 skip[4], bias[4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      skip[i] = FWD && i < en && p.D.ptr != nullptr ? ld_any(p.D.ptr, w.c0 + ec + i, p.D.dtype) : 0.0f;
-      bias[i] = i < en && p.dt_bias.ptr != nullptr ? ld_any(p.dt_bias.ptr, w.c0 + ec + i, p.dt_bias.dtype) : 0.0f;
+      const float d = FWD && i < en && p.D.ptr != nullptr ? ld_any(p.D.ptr, w.c0 + ec + i, p.D.dtype) : 0.0f;
+      const float b = i < en && p.dt_bias.ptr != nullptr ? ld_any(p.dt_bias.ptr, w.c0 + ec + i, p.dt_bias.dtype) : 0.0f;
+      (i % 2 ? skip[i / 2].y : skip[i / 2].x) = d;
+      (i % 2 ? bias[i / 2].y : bias[i / 2].x) = b;
     }
+    const bool out_vec = (p.dim * sizeof(T)) % 16 == 0 && (w.c0 * sizeof(T)) % 16 == 0;
+    T* const out = static_cast<T*>(p.out) + (static_cast<int64_t>(w.b) * p.seqlen + er) * p.dim + w.c0 + ec;
 
     auto fetch = [&](int it) {
       const int st = it % kSsmStages, t = tile_start(w, tiles, it);
@@ -116,24 +120,28 @@ struct Scan {
         x0 = read8<T>(&s.raw[st][0][0][tid], kSsmHalf);
         z0 = read8<T>(&s.raw[st][2][0][tid], kSsmHalf);
         if (er < kTokens) {
-          float v[8], u[8];
-          unpack8(read8<T>(&s.raw[st][1][0][tid], kSsmHalf), v), unpack8(x0, u);
+          float4* const dst = &s.du[st][er][ec >> 1];
+          const int turn = ec >> 4 & 3;
           // Padding takes no step and has no input; neither has what lies outside the piece.
-          const bool in = work && t + er < w.t1 && !(SEQ && ((seq.pad >> er) & 1u));
-          if (BACK && has_z) {
-            float z[8];
-            unpack8(z0, z);
+          if (work && t + er < w.t1 && !(SEQ && ((seq.pad >> er) & 1u))) {
+            float2 v[4], u[4];
+            unpack8(read8<T>(&s.raw[st][1][0][tid], kSsmHalf), v), unpack8(x0, u);
+            if (BACK && has_z) {
+              float2 z[4];
+              unpack8(z0, z);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] *= z[i] * sigmoid(z[i]);
-          }
+              for (int i = 0; i < 4; ++i) u[i] = fmul2(u[i], fmul2(z[i], sigmoid2(z[i])));
+            }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float2 delta = fadd2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(bias[2 * i], bias[2 * i + 1]));
-            if (p.softplus) delta = softplus2(delta);
-            float2 second = make_float2(u[2 * i], u[2 * i + 1]);
-            if (!BACK) second = fmul2(delta, second);
-            s.du[st][er][(ec >> 1) + (i ^ (ec >> 4 & 3))] =
-                in ? make_float4(delta.x, delta.y, second.x, second.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < 4; ++i) {
+              float2 delta = fadd2(v[i], bias[i]);
+              if (p.softplus) delta = softplus2(delta);
+              const float2 second = BACK ? u[i] : fmul2(delta, u[i]);
+              dst[i ^ turn] = make_float4(delta.x, delta.y, second.x, second.y);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
 #pragma unroll
@@ -152,23 +160,21 @@ struct Scan {
         if constexpr (FWD) {
           const int t = tile_start(w, tiles, it - 2);
           if (work && t + er < w.t1) {
-            float x[8], o[8];
-            unpack8(x2, x);
+            float2 x[4], o[4];
+            unpack8(x2, x), pairs8(&s.ys[back][er][ec], o);
 #pragma unroll
-            for (int i = 0; i < 8; i += 4) *reinterpret_cast<float4*>(&o[i]) = *reinterpret_cast<const float4*>(&s.ys[back][er][ec + i]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = fmaf(skip[i], x[i], o[i]);
+            for (int i = 0; i < 4; ++i) o[i] = ffma2(skip[i], x[i], o[i]);
             if (has_z) {
-              unpack8(z2, x);
+              float2 z[4];
+              unpack8(z2, z);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) o[i] *= x[i] * sigmoid(x[i]);
+              for (int i = 0; i < 4; ++i) o[i] = fmul2(o[i], fmul2(z[i], sigmoid2(z[i])));
             }
-            if (SEQ) {
+            if (SEQ && ((off2 >> er) & 1u)) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) o[i] = (off2 >> er) & 1u ? 0.0f : o[i];
+              for (int i = 0; i < 4; ++i) o[i] = make_float2(0.f, 0.f);
             }
-            T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(w.b) * p.seqlen + t + er) * p.dim + w.c0 + ec;
-            store8(dst, o, en, (p.dim * sizeof(T)) % 16 == 0 && (w.c0 * sizeof(T)) % 16 == 0);
+            store8(out + static_cast<int64_t>(t) * p.dim, o, en, out_vec);
           }
         }
       }
@@ -195,11 +201,14 @@ struct Scan {
         v[m] = 0.0f;
         if (in && from_init && start.ptr != nullptr)
           v[m] = ld_any(start.ptr, (static_cast<int64_t>(w.b) * p.dim + ch) * p.dstate + n0 + m, start.dtype);
-        if (FWD && in && !from_init) v[m] = p.seg_in[(piece + ch) * NP + n0 + m];
       }
       A2[c][0] = make_float2(a[0], a[1]), A2[c][1] = make_float2(a[2], a[3]);
       h[c][0] = make_float2(v[0], v[1]), h[c][1] = make_float2(v[2], v[3]);
     }
+    if (FWD && w.seg > 0) piece_in(p, w, NP, w.c0 + lc, n0, n0 + 2, false, h);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      if (lc + c >= w.nc) h[c][0] = h[c][1] = make_float2(0.f, 0.f);  // no channel
     float sum_delta[2] = {0.0f, 0.0f};
     bool cut = false;  // a sequence starts in the piece: nothing passes through it
     const int64_t kept_tiles = (p.seqlen + kSsmTile - 1) / kSsmTile;
