@@ -337,12 +337,15 @@ struct Bwd {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
           e[j][4 * m] = dB[m].x, e[j][4 * m + 1] = dB[m].y, e[j][4 * m + 2] = dC[m].x, e[j][4 * m + 3] = dC[m].y;
-        // The lane across NL holds the pairs the other way round: its second is this lane's first.
+      }
+      // The sums of the whole run together, so that the shuffles of one token do not wait for each other. The
+      // lane across NL holds the pairs of states the other way round: its second is this lane's first.
+#pragma unroll
+      for (int j = 0; j < kRun; ++j)
 #pragma unroll
         for (int k = 0; k < 4; ++k) e[j][k] += __shfl_xor_sync(0xffffffffu, e[j][4 + k], NL);
-        lane_sums<4, CL / 2, 2 * NL>(e[j]);
-        if (j % 2 == 0) lane_sums<12, NL, 1>(v[j / 2]);
-      }
+      lane_sums_of<12, NL, 1>(v);
+      lane_sums_of<4, CL / 2, 2 * NL>(e);
       static_assert(share_size<12, NL>() == 3, "each of four lanes gets three sums of a token's channel");
       __syncwarp();  // every lane has read the run's dy
 #pragma unroll

@@ -232,6 +232,31 @@ __device__ __forceinline__ void lane_sums(float (&v)[N]) {
   }
 }
 
+// The same for K sets of values side by side, stage by stage, so that their shuffles overlap.
+template <int V, int L, int BIT, int K, int N>
+__device__ __forceinline__ void lane_sums_of(float (&v)[K][N]) {
+  if constexpr (L > 1) {
+    if constexpr (V % 2 == 0) {
+      const bool up = (threadIdx.x & BIT) != 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          const float send = up ? v[k][i] : v[k][i + V / 2];
+          const float keep = up ? v[k][i + V / 2] : v[k][i];
+          v[k][i] = keep + __shfl_xor_sync(0xffffffffu, send, BIT);
+        }
+      lane_sums_of<V / 2, L / 2, 2 * BIT>(v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[k][i] += __shfl_xor_sync(0xffffffffu, v[k][i], BIT);
+      lane_sums_of<V, L / 2, 2 * BIT>(v);
+    }
+  }
+}
+
 // Position of this lane's share among the V values that lane_sums started from, and its length.
 template <int V, int L, int BIT>
 __device__ __forceinline__ int lane_share() {
