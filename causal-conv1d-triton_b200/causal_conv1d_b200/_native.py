@@ -91,7 +91,7 @@ SIGNATURES = {
                         _I, _P], _I),
     "cc1d_copy_channels": ([_P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I, _P], _I),
     "cc1d_ssm_kept_bytes": ([_I64, _I64, _I64, _I64], _I64),
-    "cc1d_ssm_workspace_bytes": ([_I64, _I64, _I64, _I64, _I64, _I], _I64),
+    "cc1d_ssm_workspace_bytes": ([_I64, _I64, _I64, _I64, _I64, _I, _I], _I64),
     "cc1d_ssm_fwd": ([_PROBLEM, _P, _P, _P, _P, _I, _I64, _P, _I64, _P, _I64, _P], _I),
     "cc1d_ssm_bwd": ([_PROBLEM, ctypes.POINTER(Tokens), _P, ctypes.POINTER(Param), ctypes.POINTER(SsmGrads), _P,
                       _I64, _P], _I),

@@ -36,20 +36,24 @@ struct Plan {
 // units of a token of one CTA alone on its SM. Measured at 64 channels of 16 states a CTA and 2048 tokens:
 // a forward takes 150 us with one CTA on every SM and 239 with two (`full`), a backward 434 and 711; the
 // pass over the pieces takes 0.75 and 0.28 of the pass it prepares (`pass`); its launch and the pieces'
-// start 7 us (`launches`).
-Plan make_plan(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t groups, bool backward, int sms) {
-  const double pass = backward ? 0.28 : 0.75, launches = backward ? 35 : 100, full = backward ? 1.64 : 1.59;
+// start 7 us (`launches`), and filling and draining a CTA's tiles 3 us (`fill`). Shared memory holds two
+// CTAs an SM except in the backward of 32-bit operands or of more than 32 states.
+Plan make_plan(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t groups, int x_dtype, bool backward,
+               int sms) {
+  const double pass = backward ? 0.28 : 0.75, launches = backward ? 35 : 100, fill = backward ? 15 : 40;
+  const double full = backward ? 1.64 : 1.59;
   Plan r;
   r.nl = ssm_lanes(static_cast<int>(dstate));
   r.blocks = static_cast<int>(cdiv(dim / groups, ssm_channels(r.nl)));
   r.segs = 1, r.seg_len = static_cast<int>(std::max<int64_t>(32, cdiv(seqlen, 32) * 32));
-  const int64_t ctas = batch * groups * r.blocks, room = 2 * sms;
+  const bool alone = backward && (x_dtype == kF32 || r.nl > 8);
+  const int64_t ctas = batch * groups * r.blocks, room = (alone ? 1 : 2) * sms;
   const int64_t most = std::min<int64_t>(cdiv(4 * room, std::max<int64_t>(1, ctas)), cdiv(seqlen, 32));
   double best = -1;
   for (int64_t want = 1; want <= std::max<int64_t>(1, most); ++want) {
     const int64_t len = cdiv(cdiv(seqlen, want), 32) * 32, segs = cdiv(seqlen, len), n = ctas * segs, rest = n % room;
-    const double waves = static_cast<double>(n / room) * full + (rest == 0 ? 0 : rest <= sms ? 1 : full);
-    const double cost = len * waves * (segs > 1 ? 1 + pass : 1) + (segs > 1 ? launches : 0);
+    const double waves = static_cast<double>(n / room) * (alone ? 1 : full) + (rest == 0 ? 0 : rest <= sms ? 1 : full);
+    const double cost = (len + fill) * waves * (segs > 1 ? 1 + pass : 1) + (segs > 1 ? launches : 0);
     if (best < 0 || cost < best) best = cost, r.segs = static_cast<int>(segs), r.seg_len = static_cast<int>(len);
   }
   return r;
@@ -61,7 +65,8 @@ int check_sizes(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int6
   return dstate > kSsmMaxState ? CC1D_ERR_UNSUPPORTED : CC1D_OK;
 }
 
-int plan_for(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t groups, bool backward, Plan* plan) {
+int plan_for(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t groups, int x_dtype, bool backward,
+             Plan* plan) {
   int sms = 0;
   const int rc = device_sms(&sms);
   if (rc != CC1D_OK) return rc;
@@ -72,12 +77,12 @@ int plan_for(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t
   };
   thread_local Known known[8] = {};
   thread_local unsigned next = 0;
-  const int64_t key[6] = {batch, seqlen, dim, dstate, 2 * groups + (backward ? 1 : 0), sms};
+  const int64_t key[6] = {batch, seqlen, dim, dstate, (groups * 4 + x_dtype) * 2 + (backward ? 1 : 0), sms};
   bool found = false;
   for (const Known& k : known)
     if (k.plan.segs > 0 && std::equal(key, key + 6, k.key)) *plan = k.plan, found = true;
   if (!found) {
-    *plan = make_plan(batch, seqlen, dim, dstate, groups, backward, sms);
+    *plan = make_plan(batch, seqlen, dim, dstate, groups, x_dtype, backward, sms);
     Known& k = known[next++ % 8];
     std::copy(key, key + 6, k.key), k.plan = *plan;
   }
@@ -161,11 +166,11 @@ int64_t cc1d_ssm_kept_bytes(int64_t batch, int64_t seqlen, int64_t dim, int64_t 
 }
 
 int64_t cc1d_ssm_workspace_bytes(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t groups,
-                                 int backward) {
-  if (check_sizes(batch, seqlen, dim, dstate, groups) != CC1D_OK) return -1;
+                                 int x_dtype, int backward) {
+  if (check_sizes(batch, seqlen, dim, dstate, groups) != CC1D_OK || !valid_dtype(x_dtype)) return -1;
   if (batch == 0 || dim == 0 || seqlen == 0) return 0;
   Plan plan;
-  if (plan_for(batch, seqlen, dim, dstate, groups, backward != 0, &plan) != CC1D_OK) return -1;
+  if (plan_for(batch, seqlen, dim, dstate, groups, x_dtype, backward != 0, &plan) != CC1D_OK) return -1;
   return 4 * (backward ? bwd_floats(plan, batch, seqlen, dim, groups) : pieces_floats(plan, batch, dim));
 }
 
@@ -178,7 +183,7 @@ int cc1d_ssm_fwd(const cc1d_ssm_problem* q, void* out, float* final_states, floa
   if (empty(*q)) return CC1D_OK;
   if (!out) return CC1D_ERR_INVALID;
   Plan plan;
-  CC1D_TRY(plan_for(q->batch, q->seqlen, q->dim, q->dstate, q->groups, false, &plan));
+  CC1D_TRY(plan_for(q->batch, q->seqlen, q->dim, q->dstate, q->groups, q->x_dtype, false, &plan));
   const int64_t need = pieces_floats(plan, q->batch, q->dim);
   if (need > 0 && (!workspace || workspace_bytes < 4 * need)) return CC1D_ERR_WORKSPACE;
   SsmParams p = common(*q, plan);
@@ -205,7 +210,7 @@ int cc1d_ssm_bwd(const cc1d_ssm_problem* q, const cc1d_tokens* dout, const float
       (grads->dinitial_states && !q->initial_states.ptr))
     return CC1D_ERR_INVALID;
   Plan plan;
-  CC1D_TRY(plan_for(q->batch, q->seqlen, q->dim, q->dstate, q->groups, true, &plan));
+  CC1D_TRY(plan_for(q->batch, q->seqlen, q->dim, q->dstate, q->groups, q->x_dtype, true, &plan));
   if (!workspace || workspace_bytes < 4 * bwd_floats(plan, q->batch, q->seqlen, q->dim, q->groups))
     return CC1D_ERR_WORKSPACE;
   SsmParams p = common(*q, plan);

@@ -163,7 +163,7 @@ std::tuple<int, at::Tensor, Opt, Opt> ssm_fwd(const at::Tensor& x, const at::Ten
     if (bytes < 0) return {q.dstate > 64 ? CC1D_ERR_UNSUPPORTED : CC1D_ERR_INVALID, out, final, kept};
     kept = floats(x, bytes);
   }
-  const int64_t ws = cc1d_ssm_workspace_bytes(q.batch, q.seqlen, q.dim, q.dstate, q.groups, 0);
+  const int64_t ws = cc1d_ssm_workspace_bytes(q.batch, q.seqlen, q.dim, q.dstate, q.groups, q.x_dtype, 0);
   at::Tensor workspace;
   if (ws > 0) workspace = floats(x, ws);
   const int rc = cc1d_ssm_fwd(&q, out.data_ptr(), final.has_value() ? final->data_ptr<float>() : nullptr,
@@ -224,7 +224,7 @@ struct SsmFn : public torch::autograd::Function<SsmFn> {
       const cc1d_param df = param(dfinal);
       auto p = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
       const cc1d_ssm_grads out{p(dx), p(ddt), p(dz), p(dB), p(dC), p(dA), p(dD), p(dbias), p(dinit)};
-      const int64_t ws = cc1d_ssm_workspace_bytes(q.batch, q.seqlen, q.dim, q.dstate, q.groups, 1);
+      const int64_t ws = cc1d_ssm_workspace_bytes(q.batch, q.seqlen, q.dim, q.dstate, q.groups, q.x_dtype, 1);
       const at::Tensor workspace = floats(x, ws);
       const int rc = cc1d_ssm_bwd(&q, &g, s[10].data_ptr<float>(), &df, &out, workspace.data_ptr(), ws, stream_of(x));
       TORCH_CHECK(rc == CC1D_OK, reason(rc, "ssm_scan backward"));

@@ -239,7 +239,8 @@ int64_t cc1d_ssm_kept_bytes(int64_t batch, int64_t seqlen, int64_t dim, int64_t 
 
 /* Bytes of the workspace of cc1d_ssm_fwd (backward 0) or cc1d_ssm_bwd (1) on the current device; -1
  * for invalid sizes. 0 for a forward that runs in one piece. */
-int64_t cc1d_ssm_workspace_bytes(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t groups, int backward);
+int64_t cc1d_ssm_workspace_bytes(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t groups,
+                                 int x_dtype, int backward);
 
 /*
  * Forward over a sequence.
@@ -249,7 +250,7 @@ int64_t cc1d_ssm_workspace_bytes(int64_t batch, int64_t seqlen, int64_t dim, int
  *   packed_state  (n_slots, dim, dstate) or NULL: with seq_idx, h after the last token of sequence id i of
  *                 row b goes to slot packed_slots[b * packed_slots_n + i]; ids at or above packed_slots_n
  *                 and slots outside [0, n_slots) are skipped
- *   workspace     at least cc1d_ssm_workspace_bytes(..., 0) bytes
+ *   workspace     at least cc1d_ssm_workspace_bytes(..., x_dtype, 0) bytes
  */
 int cc1d_ssm_fwd(const cc1d_ssm_problem* problem, void* out, float* final_states, float* kept_states,
                  void* packed_state, int packed_state_dtype, int64_t n_slots, const int32_t* packed_slots,
@@ -264,7 +265,7 @@ typedef struct cc1d_ssm_grads {
 
 /*
  * Backward. kept_states as the forward of the same problem left it; dfinal_states (batch, dim, dstate)
- * or NULL; workspace at least cc1d_ssm_workspace_bytes(..., 1) bytes. All sums over tokens, channels and
+ * or NULL; workspace at least cc1d_ssm_workspace_bytes(..., x_dtype, 1) bytes. All sums over tokens, channels and
  * CTAs are in a fixed order: the same inputs give the same bits.
  */
 int cc1d_ssm_bwd(const cc1d_ssm_problem* problem, const cc1d_tokens* dout, const float* kept_states,

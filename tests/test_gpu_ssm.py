@@ -97,18 +97,20 @@ def test_packed(dtype, dim, dstate, groups, init):
 
 
 def pieces(ops, backward):
+    """How many pieces the sequence is cut in, from the workspace that they need (cc1d_ssm_api.cu)."""
     from causal_conv1d_b200 import _native
 
     b, t, d = ops["x"].shape
-    groups = ops["B"].shape[2] if ops["B"].ndim == 4 else 1
-    ws = _native.lib.cc1d_ssm_workspace_bytes(b, t, d, ops["A"].shape[1], groups, int(backward))
-    np = 4 * (4 if ops["A"].shape[1] <= 16 else 8 if ops["A"].shape[1] <= 32 else 16)
+    n, groups = ops["A"].shape[1], ops["B"].shape[2] if ops["B"].ndim == 4 else 1
+    floats = _native.lib.cc1d_ssm_workspace_bytes(b, t, d, n, groups, _native.DTYPE_CODE[ops["x"].dtype], int(backward)) // 4
+    wide = 16 if n <= 16 else 32 if n <= 32 else 64  # states as the kernels hold them
+    piece = 3 * b * d * wide
     if not backward:
-        return max(1, ws // 4 // (2 * b * d * np))
-    blocks = groups * -(-(d // groups) // (512 * 4 // np))
-    rest = ws // 4 - b * t * blocks * 2 * np
-    one = b * (d * np + 2 * d)
-    return 1 if rest == one else (rest // (one + 2 * b * d * np))
+        return max(1, floats // piece)
+    blocks = -(-(d // groups) // (1024 // wide))
+    floats -= b * t * groups * blocks * 2 * wide
+    part = b * d * wide + 2 * b * d
+    return 1 if floats == part else floats // (part + piece)
 
 
 @pytest.mark.parametrize("kw", [dict(init=True), dict(lengths=[[300, 1, 255, -44, 424, -7, 469]])])
@@ -118,6 +120,27 @@ def test_sequence_in_pieces(dim, dstate, dtype, kw):
     ops = ref.case(5, 1, 1500, dim, dstate, 0, dtype, **kw)
     assert pieces(ops, False) > 2 and pieces(ops, True) > 2
     check_scan(ops)
+
+
+def test_one_group_does_not_reach_another():
+    """Infinities in one group's channels stay out of the other's, whose last block of channels is not full,
+    also where a gradient passes between pieces."""
+    from causal_conv1d_b200 import ssm_scan
+
+    for seqlen in (40, 1200):
+        ops = to_dev(ref.case(83, 1, seqlen, 48, 16, 2))
+        names = ("x", "dt", "B", "C", "z")
+
+        def run(dout):
+            o = {k: v.clone().requires_grad_(True) if k in names else v for k, v in ops.items()}
+            return torch.autograd.grad(ssm_scan(**o, dt_softplus=True), [o[k] for k in names], dout)
+
+        dout = torch.randn(1, seqlen, 48, device=DEV)
+        clean = run(dout)
+        dout[..., 24:] = float("inf")
+        for k, a, e in zip(names, run(dout), clean):
+            half = (slice(None), slice(None), slice(0, 1)) if k in "BC" else (Ellipsis, slice(0, 24))
+            assert torch.equal(a[half], e[half]), k
 
 
 def test_gradients_match_differences():
@@ -434,7 +457,7 @@ def test_c_abi_through_ctypes():
     for k in ("A", "D", "dt_bias", "initial_states"):
         setattr(q, k, n.Param(ops[k].data_ptr(), 0))
     out, fin = torch.empty_like(want), torch.empty_like(final)
-    size = n.lib.cc1d_ssm_workspace_bytes(2, 40, 24, 16, 2, 0)
+    size = n.lib.cc1d_ssm_workspace_bytes(2, 40, 24, 16, 2, 2, 0)
     ws = torch.empty(max(1, size), device=DEV, dtype=torch.uint8)
     stream = torch.cuda.current_stream().cuda_stream
     n.check(n.lib.cc1d_ssm_fwd(ctypes.byref(q), out.data_ptr(), fin.data_ptr(), None, None, 0, 0, None, 0,

@@ -110,7 +110,8 @@ def test_c_entry_points_refuse_before_any_device_work():
     assert lib.cc1d_ssm_update(problem(batch=3), None, 0, 2, None, None, None) == bad  # fewer slots than rows
     assert lib.cc1d_ssm_kept_bytes(1, 17, 8, 16) == 2 * 8 * 16 * 4
     assert lib.cc1d_ssm_kept_bytes(1, 17, 8, 65) == -1
-    assert lib.cc1d_ssm_workspace_bytes(1, 8, 7, 4, 2, 0) == -1
-    assert lib.cc1d_ssm_workspace_bytes(0, 8, 8, 4, 2, 1) == 0
+    assert lib.cc1d_ssm_workspace_bytes(1, 8, 7, 4, 2, 0, 0) == -1
+    assert lib.cc1d_ssm_workspace_bytes(1, 8, 8, 4, 2, 7, 0) == -1
+    assert lib.cc1d_ssm_workspace_bytes(0, 8, 8, 4, 2, 2, 1) == 0
     assert lib.cc1d_slot_maps(None, 2, 8, 1, None, None, None, 0, None, None, None, None, None, None, None) == bad
     assert lib.cc1d_slot_maps(None, -1, 8, 1, None, None, None, 0, None, None, None, None, None, None, None) == bad
