@@ -36,11 +36,11 @@ struct Plan {
 // units of a token of one CTA alone on its SM. Measured at 64 channels of 16 states a CTA and 2048 tokens:
 // a forward takes 150 us with one CTA on every SM and 239 with two (`full`), a backward 434 and 711; the
 // pass over the pieces takes 0.75 and 0.28 of the pass it prepares (`pass`); its launch and the pieces'
-// start 7 us (`launches`), and filling and draining a CTA's tiles 3 us (`fill`). Shared memory holds two
+// start 7 us (`launches`), and filling and draining a CTA's tiles 1 us (`fill`). Shared memory holds two
 // CTAs an SM except in the backward of 32-bit operands or of more than 32 states.
 Plan make_plan(int64_t batch, int64_t seqlen, int64_t dim, int64_t dstate, int64_t groups, int x_dtype, bool backward,
                int sms) {
-  const double pass = backward ? 0.28 : 0.75, launches = backward ? 35 : 100, fill = backward ? 15 : 40;
+  const double pass = backward ? 0.28 : 0.75, launches = backward ? 35 : 100, fill = backward ? 4 : 15;
   const double full = backward ? 1.64 : 1.59;
   Plan r;
   r.nl = ssm_lanes(static_cast<int>(dstate));
