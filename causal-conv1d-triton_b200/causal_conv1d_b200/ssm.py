@@ -61,7 +61,7 @@ def ssm_scan(
         for one row); ids without an entry and negative slots are skipped. Not differentiable
 
     Returns out of x's shape and dtype, or (out, final_states). Every floating input but ssm_state
-    gets a gradient; the gradients are deterministic. The forward keeps h before every 16th token
+    gets a gradient; the gradients are deterministic, and not differentiable themselves. The forward keeps h before every 16th token
     for the backward (4 * dstate / 16 bytes per element of x, dstate rounded up to 16, 32 or 64).
     """
     return tex.ssm_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, seq_idx, initial_states, return_final_states,

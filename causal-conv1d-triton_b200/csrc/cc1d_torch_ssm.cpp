@@ -197,6 +197,7 @@ struct SsmFn : public torch::autograd::Function<SsmFn> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "ssm_scan: gradients of its gradients are not available (create_graph=True)");
     const auto s = ctx->get_saved_variables();
     const at::Tensor &x = s[0], &dt = s[1], &A = s[2], &B = s[3], &C = s[4];
     auto opt = [](const at::Tensor& t) { return t.defined() ? Opt(t) : c10::nullopt; };

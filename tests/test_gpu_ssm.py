@@ -348,6 +348,59 @@ def test_same_bits_twice_and_on_another_stream():
         assert torch.equal(a, e)
 
 
+def test_second_derivatives_are_refused():
+    from causal_conv1d_b200 import ssm_scan
+
+    ops = to_dev(ref.case(79, 1, 8, 16, 4))
+    ops["x"].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="gradients of its gradients"):
+        torch.autograd.grad(ssm_scan(**ops).sum(), ops["x"], create_graph=True)
+
+
+def test_scan_in_a_graph():
+    """A captured forward and backward, in one piece and in several, replayed on new inputs."""
+    from causal_conv1d_b200 import ssm_scan
+
+    for seqlen in (40, 1000):
+        ops = to_dev(ref.case(89, 1, seqlen, 64, 16, dtype=BF16, init=True))
+        names = [k for k in GRADS if ops[k] is not None]
+        dout = torch.randn(1, seqlen, 64, device=DEV).to(BF16)
+        leaves = {k: ops[k].clone().requires_grad_(True) for k in names}
+
+        def step():
+            out, fin = ssm_scan(**{**ops, **leaves}, dt_softplus=True, return_final_states=True)
+            return (out, fin, *torch.autograd.grad([out], list(leaves.values()), [dout]))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = step()
+        with torch.no_grad():
+            leaves["x"].copy_(torch.randn(1, seqlen, 64, device=DEV).to(BF16))
+            dout.copy_(torch.randn(1, seqlen, 64, device=DEV).to(BF16))
+        graph.replay()
+        for a, e in zip(captured, step()):
+            assert torch.equal(a, e)
+
+
+def test_many_rows():
+    """More batch rows than a grid's second and third dimensions hold."""
+    from causal_conv1d_b200 import ssm_scan, ssm_update
+
+    ops = to_dev(ref.case(97, 70000, 2, 8, 4))
+    out, fin = ssm_scan(**ops, dt_softplus=True, return_final_states=True)
+    wout, wh = ref.scan(**ref.wide(ops), dt_softplus=True)
+    ref.assert_near(out, wout, 2)
+    ref.assert_near(fin, wh[:, -1], 2)
+    state = torch.zeros(70000, 8, 4, device=DEV)
+    assert torch.equal(ssm_update(ssm_state=state, dt_softplus=True, **token_ops(ops, slice(0, 2))), out)
+    assert torch.equal(state, fin)
+
+
 def token_ops(ops, t):
     return {k: v[:, t] if k in ("x", "dt", "B", "C", "z") and v is not None else v for k, v in ops.items()
             if k not in ("seq_idx", "initial_states")}
