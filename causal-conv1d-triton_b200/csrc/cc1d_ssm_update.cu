@@ -136,7 +136,10 @@ __global__ void __launch_bounds__(256, 4) cc1d_ssm_step_kernel(const __grid_cons
 }
 
 // Any number of tokens, states and alignment, four rows a CTA. VEC: a lane's 4 states are one aligned
-// vector, and so are its B and C.
+// vector, and so are its B and C. 256 rows of 4352 channels, 16 states, inputs partly in L2: 78 us for 4
+// tokens (113 with a token's operands loaded where they are used and addressed by products), 131 us for
+// 8 (202): what bounds it is the issue and latency of a token's work at 16 warps an SM (125 registers).
+// Three CTAs an SM spill, and are slower but for the longest calls (77 and 124; 21 against 19 at 64 rows).
 template <typename T, typename ST, int NL, bool VEC>
 __global__ void __launch_bounds__(256, 2) cc1d_ssm_update_kernel(const __grid_constant__ SsmUpdateParams p) {
   const int nl = threadIdx.x % NL, n0 = 4 * nl;
@@ -145,26 +148,29 @@ __global__ void __launch_bounds__(256, 2) cc1d_ssm_update_kernel(const __grid_co
   const bool in = ch < p.dim;
   const int nn = in ? p.dstate - n0 : 0;  // states of this lane
 
-  // The rows' states; null for a padded entry, of which nothing is read or written.
-  ST* st[kRows];
+  // Slots of the rows; -1 for a padded entry, of which nothing is read or written, and past the last channel.
+  int slot[kRows];
   float2 h[kRows][2];
+  ST* const state = static_cast<ST*>(p.state) + static_cast<int64_t>(ch) * p.dstate + n0;
+  const int64_t slot_size = static_cast<int64_t>(p.dim) * p.dstate;
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int b = b0 + r;
-    const int64_t slot = b >= p.batch ? -1 : (p.indices != nullptr ? p.indices[b] : b);
-    st[r] = in && slot >= 0 && slot < p.slots ? static_cast<ST*>(p.state) + (slot * p.dim + ch) * p.dstate + n0 : nullptr;
+    const int v = b >= p.batch ? -1 : (p.indices != nullptr ? p.indices[b] : b);
+    slot[r] = in && v < p.slots ? v : -1;
   }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     h[r][0] = h[r][1] = make_float2(0.f, 0.f);
-    if (st[r] != nullptr) {
+    if (slot[r] >= 0) {
+      ST* const at = state + slot[r] * slot_size;
       if (VEC) {
-        if (nn > 0) load_vec<ST, 4>(st[r], h[r]);
+        if (nn > 0) load_vec<ST, 4>(at, h[r]);
       } else {
-        if (nn > 0) h[r][0].x = to_f<ST>(st[r][0]);
-        if (nn > 1) h[r][0].y = to_f<ST>(st[r][1]);
-        if (nn > 2) h[r][1].x = to_f<ST>(st[r][2]);
-        if (nn > 3) h[r][1].y = to_f<ST>(st[r][3]);
+        if (nn > 0) h[r][0].x = to_f<ST>(at[0]);
+        if (nn > 1) h[r][0].y = to_f<ST>(at[1]);
+        if (nn > 2) h[r][1].x = to_f<ST>(at[2]);
+        if (nn > 3) h[r][1].y = to_f<ST>(at[3]);
       }
     }
   }
@@ -178,28 +184,44 @@ __global__ void __launch_bounds__(256, 2) cc1d_ssm_update_kernel(const __grid_co
   const int64_t ob = b0 + own;
   bool own_live = false;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) own_live = r == own ? st[r] != nullptr : own_live;
+  for (int r = 0; r < kRows; ++r) own_live = r == own ? slot[r] >= 0 : own_live;
   const int64_t g = in ? ch / p.group_dim : 0;
-  const T* bp = static_cast<const T*>(p.Bm.ptr) + g * p.Bm.sg;
-  const T* cp = static_cast<const T*>(p.Cm.ptr) + g * p.Cm.sg;
+  const T* bp = static_cast<const T*>(p.Bm.ptr) + b0 * p.Bm.sb + g * p.Bm.sg;
+  const T* cp = static_cast<const T*>(p.Cm.ptr) + b0 * p.Cm.sb + g * p.Cm.sg;
+  const T* xp = static_cast<const T*>(p.x.ptr) + ob * p.x.sb + ch;
+  const T* dp = static_cast<const T*>(p.dt.ptr) + ob * p.dt.sb + ch;
+  const T* zp = static_cast<const T*>(p.z.ptr) + ob * p.z.sb + ch;
+  T* op = static_cast<T*>(p.out) + ob * p.seqlen * p.dim + ch;
 
-#pragma unroll 1
-  for (int64_t l = 0; l < p.seqlen; ++l) {
-    float x = 0.0f, delta = 0.0f, z = 0.0f;
+  // A token's operands are on the way while the token before it is computed.
+  T xt = from_f<T>(0.0f), dtt = xt, zt = xt;
+  Raw4<T> Bt[kRows], Ct[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) Bt[r] = Ct[r] = zero4<T>();
+  auto fetch = [&]() {
     if (own_live) {
-      x = to_f<T>(static_cast<const T*>(p.x.ptr)[ob * p.x.sb + l * p.x.st + ch]);
-      delta = to_f<T>(static_cast<const T*>(p.dt.ptr)[ob * p.dt.sb + l * p.dt.st + ch]) + bias;
-      if (p.z.ptr != nullptr) z = to_f<T>(static_cast<const T*>(p.z.ptr)[ob * p.z.sb + l * p.z.st + ch]);
+      xt = *xp, dtt = *dp;
+      if (p.z.ptr != nullptr) zt = *zp;
     }
-    Raw4<T> B[kRows], C[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      B[r] = C[r] = zero4<T>();
-      if (st[r] != nullptr && nn > 0) {
-        B[r] = load4(bp + (b0 + r) * p.Bm.sb + l * p.Bm.st, n0, VEC ? kSsmMaxState : p.dstate, VEC);
-        C[r] = load4(cp + (b0 + r) * p.Cm.sb + l * p.Cm.st, n0, VEC ? kSsmMaxState : p.dstate, VEC);
+      if (slot[r] >= 0 && nn > 0) {
+        Bt[r] = load4(bp + r * p.Bm.sb, n0, VEC ? kSsmMaxState : p.dstate, VEC);
+        Ct[r] = load4(cp + r * p.Cm.sb, n0, VEC ? kSsmMaxState : p.dstate, VEC);
       }
     }
+    xp += p.x.st, dp += p.dt.st, zp += p.z.st, bp += p.Bm.st, cp += p.Cm.st;
+  };
+  if (p.seqlen > 0) fetch();
+
+#pragma unroll 1
+  for (int64_t l = 0; l < p.seqlen; ++l, op += p.dim) {
+    const float x = own_live ? to_f<T>(xt) : 0.0f, z = to_f<T>(zt);
+    float delta = own_live ? to_f<T>(dtt) + bias : 0.0f;
+    Raw4<T> B[kRows], C[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) B[r] = Bt[r], C[r] = Ct[r];
+    if (l + 1 < p.seqlen) fetch();
     if (p.softplus) delta = softplus(delta);
     const float u = delta * x;
     float y[kRows];
@@ -218,19 +240,20 @@ __global__ void __launch_bounds__(256, 2) cc1d_ssm_update_kernel(const __grid_co
     if (own_live && nl < 4) {
       float o = fmaf(skip, x, y[0]);
       if (p.z.ptr != nullptr) o *= z * sigmoid(z);
-      static_cast<T*>(p.out)[(ob * p.seqlen + l) * p.dim + ch] = from_f<T>(o);
+      *op = from_f<T>(o);
     }
   }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    if (st[r] != nullptr) {
+    if (slot[r] >= 0) {
+      ST* const at = state + slot[r] * slot_size;
       if (VEC) {
-        if (nn > 0) store_vec<ST, 4>(st[r], h[r]);
+        if (nn > 0) store_vec<ST, 4>(at, h[r]);
       } else {
-        if (nn > 0) st[r][0] = from_f<ST>(h[r][0].x);
-        if (nn > 1) st[r][1] = from_f<ST>(h[r][0].y);
-        if (nn > 2) st[r][2] = from_f<ST>(h[r][1].x);
-        if (nn > 3) st[r][3] = from_f<ST>(h[r][1].y);
+        if (nn > 0) at[0] = from_f<ST>(h[r][0].x);
+        if (nn > 1) at[1] = from_f<ST>(h[r][0].y);
+        if (nn > 2) at[2] = from_f<ST>(h[r][1].x);
+        if (nn > 3) at[3] = from_f<ST>(h[r][1].y);
       }
     }
   }
