@@ -18,6 +18,7 @@ namespace cc1d {
 namespace {
 
 constexpr int kRows = 4;
+constexpr int kStep = 128;  // threads of a CTA of the one-token kernel
 
 // 4 consecutive elements of a buffer whose type is given at run time, the first `n` of them.
 __device__ __forceinline__ void ld_any4(const void* base, int64_t i, int dtype, int n, float (&v)[4]) {
@@ -34,15 +35,18 @@ __device__ __forceinline__ void ld_any4(const void* base, int64_t i, int dtype, 
 
 // One token of every row, dstate 16, 32 or 64, all of it in aligned vectors: what a decode step is. A CTA
 // takes G groups of kRows rows of its channels and has all their states on the way at once, as
-// asynchronous copies of each thread's own pieces (32 KB a CTA at G = 2, four CTAs an SM). 256 rows of
-// 4352 channels, fp32 states, 151 MB: 32.5 us, 0.71 of the measured copy bandwidth; 33.8 us with three
-// groups, 35.4 with four (80 registers, three CTAs), 41 with the loads of a group in registers.
+// asynchronous copies of each thread's own pieces (16 KB a CTA at G = 2, eight CTAs an SM: with 256 threads
+// and four, 128 rows of 2048 channels take 9.2 us instead of 8.5, and 256 x 4352 0.5 us more). 256 rows of
+// 4352 channels, fp32 states, 151 MB: 31.6 us between other calls, 28.5 in a row of such steps (5.3 TB/s,
+// 0.81 of the measured copy bandwidth); against 32.5 before, 33.8 us with three groups, 35.4 with four (80 registers, three
+// quarters of the threads), 41 with the loads of a group in registers. Issue slots are 69% taken (124 instructions a
+// warp and row); addresses of one 32-bit product and B and C a group ahead are no faster.
 template <typename T, typename ST, int NL, int G>
-__global__ void __launch_bounds__(256, 4) cc1d_ssm_step_kernel(const __grid_constant__ SsmUpdateParams p) {
+__global__ void __launch_bounds__(kStep, 1024 / kStep) cc1d_ssm_step_kernel(const __grid_constant__ SsmUpdateParams p) {
   constexpr int BYTES = 4 * static_cast<int>(sizeof(ST));
-  extern __shared__ __align__(16) unsigned char staged[];  // [G][kRows][256] pieces
+  extern __shared__ __align__(16) unsigned char staged[];  // [G][kRows][kStep] pieces
   const int nl = threadIdx.x % NL, n0 = 4 * nl;
-  const int own_ch = static_cast<int>(blockIdx.x % p.blocks) * (256 / NL) + static_cast<int>(threadIdx.x) / NL;
+  const int own_ch = static_cast<int>(blockIdx.x % p.blocks) * (kStep / NL) + static_cast<int>(threadIdx.x) / NL;
   const bool in = own_ch < p.dim;
   const int ch = in ? own_ch : p.dim - 1;  // lanes past the last channel compute it again, and write nothing
   const int b0 = static_cast<int>(blockIdx.x / p.blocks) * (G * kRows);
@@ -65,7 +69,7 @@ __global__ void __launch_bounds__(256, 4) cc1d_ssm_step_kernel(const __grid_cons
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
       if (slot[q][r] >= 0)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(staged) + ((q * kRows + r) * 256 + threadIdx.x) * BYTES),
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(staged) + ((q * kRows + r) * kStep + threadIdx.x) * BYTES),
                      "l"(state + slot[q][r] * slot_size), "n"(BYTES)
                      : "memory");
     copies_issued();
@@ -113,7 +117,7 @@ __global__ void __launch_bounds__(256, 4) cc1d_ssm_step_kernel(const __grid_cons
       const float2 d = splat(__shfl_sync(0xffffffffu, delta, from)), v = splat(__shfl_sync(0xffffffffu, u, from));
       const float4 b = unpack4(B[r]), c = unpack4(C[r]);
       float2 h[2];
-      load_vec<ST, 4>(reinterpret_cast<const ST*>(staged) + ((q * kRows + r) * 256 + threadIdx.x) * 4, h);
+      load_vec<ST, 4>(reinterpret_cast<const ST*>(staged) + ((q * kRows + r) * kStep + threadIdx.x) * 4, h);
       const float2 a0 = decay2<T>(fmul2(d, A2[0])), a1 = decay2<T>(fmul2(d, A2[1]));
       h[0] = ffma2(a0, h[0], fmul2(v, make_float2(b.x, b.y)));
       h[1] = ffma2(a1, h[1], fmul2(v, make_float2(b.z, b.w)));
@@ -260,12 +264,13 @@ __global__ void __launch_bounds__(256, 2) cc1d_ssm_update_kernel(const __grid_co
 }
 
 template <typename T, typename ST, int NL, int G>
-cudaError_t launch_step(const SsmUpdateParams& p, cudaStream_t s) {
-  constexpr int smem = G * kRows * 256 * 4 * static_cast<int>(sizeof(ST));
+cudaError_t launch_step(SsmUpdateParams p, cudaStream_t s) {
+  p.blocks = static_cast<int>((static_cast<int64_t>(p.dim) * NL + kStep - 1) / kStep);
+  constexpr int smem = G * kRows * kStep * 4 * static_cast<int>(sizeof(ST));
   const cudaError_t e = allow_smem<cc1d_ssm_step_kernel<T, ST, NL, G>>(smem);
   if (e != cudaSuccess) return e;
   const unsigned grid = static_cast<unsigned>(p.blocks) * ((p.batch + G * kRows - 1) / (G * kRows));
-  cc1d_ssm_step_kernel<T, ST, NL, G><<<grid, 256, smem, s>>>(p);
+  cc1d_ssm_step_kernel<T, ST, NL, G><<<grid, kStep, smem, s>>>(p);
   return cudaGetLastError();
 }
 
@@ -273,7 +278,7 @@ template <typename T, typename ST, int NL>
 cudaError_t launch(const SsmUpdateParams& p, cudaStream_t s) {
   const bool vec = p.dstate % 4 == 0 && reinterpret_cast<uintptr_t>(p.state) % (4 * sizeof(ST)) == 0 && p.Bm.vec && p.Cm.vec;
   if (vec && p.seqlen == 1 && p.dstate == 4 * NL) {
-    // Two groups a CTA where that leaves two CTAs for every SM (148), one for small batches.
+    // Two groups a CTA where that leaves 512 threads for every SM (148), one for small batches.
     const int64_t wide = static_cast<int64_t>(p.blocks) * ((p.batch + 2 * kRows - 1) / (2 * kRows));
     return wide >= 2 * 148 ? launch_step<T, ST, NL, 2>(p, s) : launch_step<T, ST, NL, 1>(p, s);
   }
