@@ -34,6 +34,7 @@ struct SsmParams {
   int softplus;
   int segs, seg_len;  // the sequence in `segs` pieces of `seg_len` tokens (a multiple of 32)
   int blocks;         // CTAs that cover one group's channels
+  int out_vec;        // out (backward: dx, ddt and dz) and the rows in it start at multiples of 16 bytes
   // Forward
   void* out;                   // (batch, seqlen, dim) contiguous, type of x
   float* final_states;         // (batch, dim, dstate) or null

@@ -2,6 +2,7 @@
 // kernels find, how a sequence is cut in pieces, and the workspaces. Declared in
 // include/causal_conv1d_b200.h.
 #include <algorithm>
+#include <initializer_list>
 
 #include "causal_conv1d_b200.h"
 #include "cc1d_device.cuh"
@@ -114,6 +115,15 @@ SsmTokens tokens(const cc1d_tokens& t, int n, int es, const cc1d_ssm_problem& q)
   return {t.ptr, t.stride_batch, t.stride_time, t.stride_group, vec};
 }
 
+// Whether every row of the contiguous outputs, `dim` elements each, starts at a multiple of 16 bytes (a null
+// output has no rows).
+int aligned_rows(int64_t dim, int es, std::initializer_list<const void*> outs) {
+  if (dim * es % 16 != 0) return 0;
+  for (const void* o : outs)
+    if (reinterpret_cast<uintptr_t>(o) % 16 != 0) return 0;
+  return 1;
+}
+
 SsmParam param(const cc1d_param& q) { return {q.ptr, q.dtype}; }
 
 int check_problem(const cc1d_ssm_problem* q) {
@@ -187,6 +197,7 @@ int cc1d_ssm_fwd(const cc1d_ssm_problem* q, void* out, float* final_states, floa
   const int64_t need = pieces_floats(plan, q->batch, q->dim);
   if (need > 0 && (!workspace || workspace_bytes < 4 * need)) return CC1D_ERR_WORKSPACE;
   SsmParams p = common(*q, plan);
+  p.out_vec = aligned_rows(q->dim, elem_size(q->x_dtype), {out});
   p.out = out, p.final_states = final_states, p.kept = kept_states;
   p.cache = packed_state, p.cache_dtype = packed_state_dtype, p.cache_idx = packed_slots, p.cache_n = packed_slots_n;
   p.cache_slots = n_slots;
@@ -217,6 +228,7 @@ int cc1d_ssm_bwd(const cc1d_ssm_problem* q, const cc1d_tokens* dout, const float
   p.dout = tokens(*dout, 8, elem_size(q->x_dtype), *q);
   if (dfinal_states) p.dfinal = param(*dfinal_states);
   p.kept = const_cast<float*>(kept_states);
+  p.out_vec = aligned_rows(q->dim, elem_size(q->x_dtype), {grads->dx, grads->ddt, q->z.ptr ? grads->dz : nullptr});
   p.dx = grads->dx, p.ddt = grads->ddt, p.dz = grads->dz, p.dB = grads->dB, p.dC = grads->dC;
   p.dA = grads->dA, p.dD = q->D.ptr ? grads->dD : nullptr, p.ddt_bias = q->dt_bias.ptr ? grads->ddt_bias : nullptr;
   p.dinit = grads->dinitial_states;

@@ -105,7 +105,7 @@ struct Bwd {
     const int br = tid / (2 * NP), bk = tid % (2 * NP);
     const int64_t bc_row = static_cast<int64_t>(p.groups) * p.blocks * (2 * NP);
     float* const part_bc = p.part_bc + (static_cast<int64_t>(w.b) * p.seqlen + br) * bc_row + (w.g * p.blocks + w.blk) * (2 * NP) + bk;
-    const bool out_vec = (p.dim * sizeof(T)) % 16 == 0 && (w.c0 * sizeof(T)) % 16 == 0;
+    const bool out_vec = p.out_vec && (w.c0 * sizeof(T)) % 16 == 0;
     const int64_t out = (static_cast<int64_t>(w.b) * p.seqlen + er) * p.dim + w.c0 + ec;
     const int turn = ec >> 4 & 3;
 

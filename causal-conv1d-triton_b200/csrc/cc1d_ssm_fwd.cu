@@ -76,7 +76,7 @@ struct Scan {
       (i % 2 ? skip[i / 2].y : skip[i / 2].x) = d;
       (i % 2 ? bias[i / 2].y : bias[i / 2].x) = b;
     }
-    const bool out_vec = (p.dim * sizeof(T)) % 16 == 0 && (w.c0 * sizeof(T)) % 16 == 0;
+    const bool out_vec = p.out_vec && (w.c0 * sizeof(T)) % 16 == 0;
     T* const out = static_cast<T*>(p.out) + (static_cast<int64_t>(w.b) * p.seqlen + er) * p.dim + w.c0 + ec;
 
     auto fetch = [&](int it) {

@@ -572,3 +572,53 @@ def test_slot_maps_lengths_that_pass_32_bits():
     assert got.seq_idx.tolist() == [[0] * 5 + [1] * 7]
     with pytest.raises(AssertionError):
         slot_maps_from_lengths(lengths, 12, slots=torch.zeros(4, dtype=torch.int32))  # not on the device
+
+
+def c_problem(ops):
+    """ops (on the device, contiguous, grouped B and C) as the header's structure."""
+    from causal_conv1d_b200 import _native as n
+
+    b, t, d = ops["x"].shape
+    q = n.SsmProblem(batch=b, seqlen=t, dim=d, dstate=ops["A"].shape[1], groups=ops["B"].shape[2],
+                     x_dtype=n.DTYPE_CODE[ops["x"].dtype], dt_softplus=1)
+    for k in ("x", "dt", "z", "B", "C"):
+        s = ops[k].stride()
+        setattr(q, k, n.Tokens(ops[k].data_ptr(), s[0], s[1], s[2] if k in "BC" else 0))
+    for k in ("A", "D", "dt_bias", "initial_states"):
+        setattr(q, k, n.Param(ops[k].data_ptr(), 0))
+    return q
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("groups", [1, 2])
+def test_c_abi_outputs_at_any_element(dtype, groups):
+    """Outputs and gradients that start at any element of a buffer: rows of 16 bytes' multiples from there on
+    have the same values as aligned ones, and their neighbours are left alone."""
+    from causal_conv1d_b200 import _native as n
+
+    ops = to_dev(ref.case(101, 2, 40, 48, 16, groups, dtype, init=True))
+    q, stream, size = c_problem(ops), torch.cuda.current_stream().cuda_stream, 2 * 40 * 48
+    dout = torch.randn(2, 40, 48, device=DEV).to(dtype)
+    dout_c = n.Tokens(dout.data_ptr(), dout.stride(0), dout.stride(1), 0)
+    work = [n.lib.cc1d_ssm_workspace_bytes(2, 40, 48, 16, groups, q.x_dtype, k) for k in (0, 1)]
+    ws = torch.empty(max(16, *work), device=DEV, dtype=torch.uint8)
+    kept = torch.empty(n.lib.cc1d_ssm_kept_bytes(2, 40, 48, 16), device=DEV, dtype=torch.uint8)
+
+    def run(offset):
+        wide = {k: torch.full((size + 16,), 7.0, device=DEV, dtype=dtype) for k in ("out", "dx", "ddt", "dz")}
+        at = {k: v.data_ptr() + offset * v.element_size() for k, v in wide.items()}
+        dB, dC, dA = torch.empty_like(ops["B"]), torch.empty_like(ops["C"]), torch.empty_like(ops["A"])
+        dD, db, di = torch.empty_like(ops["D"]), torch.empty_like(ops["dt_bias"]), torch.empty_like(ops["initial_states"])
+        grads = n.SsmGrads(at["dx"], at["ddt"], at["dz"], *(t.data_ptr() for t in (dB, dC, dA, dD, db, di)))
+        n.check(n.lib.cc1d_ssm_fwd(ctypes.byref(q), at["out"], None, kept.data_ptr(), None, 0, 0, None, 0, ws.data_ptr(),
+                                   work[0], stream), "cc1d_ssm_fwd")
+        n.check(n.lib.cc1d_ssm_bwd(ctypes.byref(q), ctypes.byref(dout_c), kept.data_ptr(), None, ctypes.byref(grads),
+                                   ws.data_ptr(), work[1], stream), "cc1d_ssm_bwd")
+        for v in wide.values():
+            assert (v[:offset] == 7).all() and (v[offset + size:] == 7).all()
+        return [v[offset:offset + size] for v in wide.values()] + [dB, dC, dA, dD, db, di]
+
+    plain = run(0)
+    for offset in (1, 2, 3):
+        for a, e in zip(run(offset), plain):
+            assert torch.equal(a, e)
