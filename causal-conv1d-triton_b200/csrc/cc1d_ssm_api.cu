@@ -155,6 +155,9 @@ void set_pieces(SsmParams& p, float* ws, int64_t floats) {
   p.seg_out = ws, p.seg_decay = ws + floats / 3, p.seg_in = ws + 2 * (floats / 3);
 }
 
+// The buffers that the kernels read and write in vectors whatever the operands' alignment.
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 int done(cudaError_t e) { return e == cudaSuccess ? CC1D_OK : record_cuda_error(e); }
 
 #define CC1D_TRY(call)              \
@@ -191,7 +194,7 @@ int cc1d_ssm_fwd(const cc1d_ssm_problem* q, void* out, float* final_states, floa
   if (packed_state && (!q->seq_idx || !packed_slots || packed_slots_n < 0 || !valid_dtype(packed_state_dtype)))
     return CC1D_ERR_INVALID;
   if (empty(*q)) return CC1D_OK;
-  if (!out) return CC1D_ERR_INVALID;
+  if (!out || !aligned16(kept_states) || !aligned16(workspace)) return CC1D_ERR_INVALID;
   Plan plan;
   CC1D_TRY(plan_for(q->batch, q->seqlen, q->dim, q->dstate, q->groups, q->x_dtype, false, &plan));
   const int64_t need = pieces_floats(plan, q->batch, q->dim);
@@ -218,7 +221,7 @@ int cc1d_ssm_bwd(const cc1d_ssm_problem* q, const cc1d_tokens* dout, const float
   if (empty(*q)) return CC1D_OK;
   if (!dout->ptr || !kept_states || !grads->dx || !grads->ddt || !grads->dA || !grads->dB || !grads->dC ||
       (q->z.ptr && !grads->dz) || (q->D.ptr && !grads->dD) || (q->dt_bias.ptr && !grads->ddt_bias) ||
-      (grads->dinitial_states && !q->initial_states.ptr))
+      (grads->dinitial_states && !q->initial_states.ptr) || !aligned16(kept_states) || !aligned16(workspace))
     return CC1D_ERR_INVALID;
   Plan plan;
   CC1D_TRY(plan_for(q->batch, q->seqlen, q->dim, q->dstate, q->groups, q->x_dtype, true, &plan));

@@ -205,7 +205,9 @@ int cc1d_copy_channels(void* dst, int64_t dst_stride_batch, int64_t dst_stride_t
  *   h[t] = exp(delta[t] A[d, n]) h[t-1] + delta[t] x[t] B[t, n]
  *   out[t] = (sum_n C[t, n] h[t] + D[d] x[t]) silu(z[t])
  *
- * All arithmetic and h are fp32; x, dt, z, B, C, out and their gradients have one element type.
+ * All arithmetic and h are fp32; x, dt, z, B, C, out and their gradients have one element type. Operands
+ * and outputs may start at any element of a buffer; kept states and workspaces start at a multiple of 16
+ * bytes, else the call returns CC1D_ERR_INVALID.
  * --------------------------------------------------------------------------------------------- */
 
 /* Element (b, t, c) at ptr + b*stride_batch + t*stride_time + c elements; for B and C, state n of

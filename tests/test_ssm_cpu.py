@@ -115,3 +115,20 @@ def test_c_entry_points_refuse_before_any_device_work():
     assert lib.cc1d_ssm_workspace_bytes(0, 8, 8, 4, 2, 2, 1) == 0
     assert lib.cc1d_slot_maps(None, 2, 8, 1, None, None, None, 0, None, None, None, None, None, None, None) == bad
     assert lib.cc1d_slot_maps(None, -1, 8, 1, None, None, None, 0, None, None, None, None, None, None, None) == bad
+
+
+def test_c_entry_points_refuse_unaligned_scratch():
+    """Kept states and workspaces move in 16-byte vectors. The addresses are never read: the refusal comes
+    before any device work."""
+    from causal_conv1d_b200 import _native as n
+
+    q = n.SsmProblem(batch=1, seqlen=8, dim=8, dstate=4, groups=1, x_dtype=2)
+    for k in ("x", "dt", "B", "C"):
+        setattr(q, k, n.Tokens(4096, 64, 8, 8))
+    q.A = n.Param(4096, 0)
+    grads = n.SsmGrads(*([4096] * 6))
+    dout = n.Tokens(4096, 64, 8, 0)
+    for kept, workspace in ((4100, 4096), (4096, 4104)):
+        assert n.lib.cc1d_ssm_fwd(ctypes.byref(q), 4096, None, kept, None, 0, 0, None, 0, workspace, 1 << 30, None) == n.CC1D_ERR_INVALID
+        assert n.lib.cc1d_ssm_bwd(ctypes.byref(q), ctypes.byref(dout), kept, None, ctypes.byref(grads), workspace, 1 << 30,
+                                  None) == n.CC1D_ERR_INVALID
