@@ -64,7 +64,7 @@ __device__ __forceinline__ void put_tokens(const SlotMapParams& p, const int32_t
       id[i] = lo < p.n ? lo : -1;
       at[i] = lo < p.n ? static_cast<int32_t>(pos + i) - edges[lo] + (p.past != nullptr ? p.past[lo] : 0) : -1;
     }
-    if (pos + 4 <= p.seqlen) {
+    if (p.vec && pos + 4 <= p.seqlen) {
       *reinterpret_cast<int4*>(p.seq_idx + pos) = make_int4(id[0], id[1], id[2], id[3]);
       *reinterpret_cast<int4*>(p.positions + pos) = make_int4(at[0], at[1], at[2], at[3]);
     } else {

@@ -10,6 +10,7 @@ struct SlotMapParams {
   const int32_t *lengths, *past, *slots, *free_slots;  // past and slots may be null
   int32_t *cu_seqlens, *seq_idx, *positions, *tail_rows, *slots_out, *n_taken;
   int n, seqlen, width;
+  int vec;  // seq_idx and positions start at multiples of 16 bytes
   int64_t n_free;
 };
 

@@ -281,6 +281,7 @@ int cc1d_slot_maps(const int32_t* lengths, int64_t n, int64_t seqlen, int64_t wi
   p.cu_seqlens = cu_seqlens, p.seq_idx = seq_idx, p.positions = positions, p.tail_rows = tail_rows;
   p.slots_out = slots_out, p.n_taken = n_taken;
   p.n = static_cast<int>(n), p.seqlen = static_cast<int>(seqlen), p.width = static_cast<int>(width);
+  p.vec = aligned16(seq_idx) && aligned16(positions);
   return done(launch_slot_maps(p, static_cast<cudaStream_t>(stream)));
 }
 

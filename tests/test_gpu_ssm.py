@@ -622,3 +622,21 @@ def test_c_abi_outputs_at_any_element(dtype, groups):
     for offset in (1, 2, 3):
         for a, e in zip(run(offset), plain):
             assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("n, seqlen", [(7, 1030), (4097, 9001)])
+def test_c_abi_slot_maps_at_any_element(n, seqlen):
+    from causal_conv1d_b200 import _native, slot_maps_from_lengths
+
+    lengths = torch.randint(0, 2 * seqlen // n, (n,), generator=torch.Generator().manual_seed(n), dtype=torch.int32).to(DEV)
+    want = slot_maps_from_lengths(lengths, seqlen, 4)
+    for a, b in ((1, 0), (0, 3), (2, 2)):
+        seq, pos = (torch.full((seqlen + 8,), 7, device=DEV, dtype=torch.int32) for _ in range(2))
+        cu, tail, taken = (torch.empty(k, device=DEV, dtype=torch.int32) for k in (n + 1, 3 * n, 1))
+        _native.check(_native.lib.cc1d_slot_maps(
+            lengths.data_ptr(), n, seqlen, 4, None, None, None, 0, cu.data_ptr(), seq.data_ptr() + 4 * a, pos.data_ptr() + 4 * b,
+            tail.data_ptr(), None, taken.data_ptr(), torch.cuda.current_stream().cuda_stream), "cc1d_slot_maps")
+        assert torch.equal(seq[a:a + seqlen], want.seq_idx[0]) and torch.equal(pos[b:b + seqlen], want.positions[0])
+        for buf, k in ((seq, a), (pos, b)):
+            assert (buf[:k] == 7).all() and (buf[k + seqlen:] == 7).all()
+        assert torch.equal(cu, want.cu_seqlens) and torch.equal(tail.view(n, 3), want.tail_rows)
