@@ -104,7 +104,8 @@ struct Bwd {
     static_assert(kSsmHalf % (2 * NP) == 0 && SUMS * kSsmHalf == kTokens * 2 * NP, "");
     const int br = tid / (2 * NP), bk = tid % (2 * NP);
     const int64_t bc_row = static_cast<int64_t>(p.groups) * p.blocks * (2 * NP);
-    float* const part_bc = p.part_bc + (static_cast<int64_t>(w.b) * p.seqlen + br) * bc_row + (w.g * p.blocks + w.blk) * (2 * NP) + bk;
+    float* const part_bc = p.part_bc + (static_cast<int64_t>(w.b) * p.seqlen + br) * bc_row +
+                           (static_cast<int64_t>(w.g) * p.blocks + w.blk) * (2 * NP) + bk;
     const bool out_vec = p.out_vec && (w.c0 * sizeof(T)) % 16 == 0;
     const int64_t out = (static_cast<int64_t>(w.b) * p.seqlen + er) * p.dim + w.c0 + ec;
     const int turn = ec >> 4 & 3;

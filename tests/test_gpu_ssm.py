@@ -640,3 +640,20 @@ def test_c_abi_slot_maps_at_any_element(n, seqlen):
         for buf, k in ((seq, a), (pos, b)):
             assert (buf[:k] == 7).all() and (buf[k + seqlen:] == 7).all()
         assert torch.equal(cu, want.cu_seqlens) and torch.equal(tail.view(n, 3), want.tail_rows)
+
+
+def test_backward_offsets_past_32_bits():
+    """So many groups that the sums of the last ones lie past 2^31: one token, so that dB is delta x dy C and
+    dC is dy delta x B."""
+    from causal_conv1d_b200 import ssm_scan
+
+    groups, n = 2**24 + 40, 33
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x, dt, dout = (torch.randn(1, 1, groups, generator=g, device=DEV).to(BF16) for _ in range(3))
+    B, C = (torch.randn(1, 1, groups, n, generator=g, device=DEV).to(BF16).requires_grad_(True) for _ in range(2))
+    A = torch.full((groups, n), -1.0, device=DEV, dtype=BF16)
+    dB, dC = torch.autograd.grad(ssm_scan(x, dt, A, B, C), [B, C], dout)
+    for part in (slice(0, 1000), slice(groups - 1000, groups)):
+        u = (dt[..., part].double() * x[..., part].double() * dout[..., part].double()).unsqueeze(-1)
+        ref.assert_near(dB[:, :, part], u * C[:, :, part].double(), 1, "dB")
+        ref.assert_near(dC[:, :, part], u * B[:, :, part].double(), 1, "dC")
