@@ -353,7 +353,7 @@ __device__ __forceinline__ SsmPlace ssm_place(const SsmParams& p) {
   w.c0 = w.g * p.group_dim + w.blk * CH;
   w.nc = min(CH, p.group_dim - w.blk * CH);
   w.t0 = w.seg * p.seg_len;
-  w.t1 = min(p.seqlen, w.t0 + p.seg_len);
+  w.t1 = w.t0 + min(p.seqlen - w.t0, p.seg_len);  // the last piece's t0 + seg_len may pass 2^31
   return w;
 }
 

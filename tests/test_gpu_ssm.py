@@ -657,3 +657,18 @@ def test_backward_offsets_past_32_bits():
         u = (dt[..., part].double() * x[..., part].double() * dout[..., part].double()).unsqueeze(-1)
         ref.assert_near(dB[:, :, part], u * C[:, :, part].double(), 1, "dB")
         ref.assert_near(dC[:, :, part], u * B[:, :, part].double(), 1, "dC")
+
+
+def test_scan_of_the_longest_row():
+    """The most tokens that the header allows, zero but for the last ones: the last of the pieces would end past
+    2^31."""
+    from causal_conv1d_b200 import ssm_scan
+
+    T, tail = 2**31 - 64, 100
+    end = to_dev(ref.case(103, 1, tail, 1, 1, dtype=BF16, D=False, z=False))
+    ops = {k: torch.zeros(1, T, 1, device=DEV, dtype=BF16) if k in ("x", "dt", "B", "C") else v for k, v in end.items()}
+    for k in ("x", "dt", "B", "C"):
+        ops[k][:, -tail:] = end[k]
+    out = ssm_scan(**ops, dt_softplus=True)
+    ref.assert_near(out[:, -tail:], ref.scan(**ref.wide(end), dt_softplus=True)[0], tail)
+    assert not out[:, :-tail].any()
