@@ -24,9 +24,14 @@ __device__ __forceinline__ float2 exp2_approx2(float2 x) { return make_float2(ex
 
 // 2^x = 2^i 2^f with i the nearest integer (found by adding and taking off 1.5 2^23) and 2^f, |f| <= 1/2, by
 // its Taylor polynomial of degree 6 (ln2^k / k!, below 2e-7 off at |f| = 1/2 and exact to rounding for small
-// f). Arguments below -126 give 2^-126, above 128 infinity; a NaN's h is NaN through its input.
+// f). Arguments below -126 give 2^-126, above 127.5 infinity. A NaN gives a NaN: it passes the limits, and the
+// power of two, which means nothing then, is multiplied and not added to the exponent's bits.
+__device__ __forceinline__ float within(float x, float lo, float hi) {
+  asm("max.NaN.f32 %0, %0, %1;\n\tmin.NaN.f32 %0, %0, %2;" : "+f"(x) : "f"(lo), "f"(hi));
+  return x;
+}
 __device__ __forceinline__ float2 exp2_exact2(float2 x) {
-  x = make_float2(fminf(fmaxf(x.x, -126.0f), 128.0f), fminf(fmaxf(x.y, -126.0f), 128.0f));
+  x = make_float2(within(x.x, -126.0f, 128.0f), within(x.y, -126.0f, 128.0f));
   const float2 t = fadd2(x, splat(12582912.0f)), f = fadd2(x, fmul2(fadd2(t, splat(-12582912.0f)), splat(-1.0f)));
   float2 q = ffma2(f, splat(1.5403530e-4f), splat(1.3333558e-3f));
   q = ffma2(q, f, splat(9.6181291e-3f));
@@ -34,8 +39,8 @@ __device__ __forceinline__ float2 exp2_exact2(float2 x) {
   q = ffma2(q, f, splat(2.4022651e-1f));
   q = ffma2(q, f, splat(6.9314718e-1f));
   q = ffma2(q, f, splat(1.0f));
-  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+  return fmul2(q, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                              __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
 }
 
 // The decay of a step, for operands of type T. A one-sided error adds up over as many tokens as a state

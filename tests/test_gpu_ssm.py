@@ -672,3 +672,37 @@ def test_scan_of_the_longest_row():
     out = ssm_scan(**ops, dt_softplus=True)
     ref.assert_near(out[:, -tail:], ref.scan(**ref.wide(end), dt_softplus=True)[0], tail)
     assert not out[:, :-tail].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("seqlen, dstate", [(40, 16), (700, 16), (40, 40)])
+def test_nan_in_a_decay_rate(dtype, seqlen, dstate):
+    """It reaches its channel's outputs, its own state and its own gradient, and no other channel or state."""
+    from causal_conv1d_b200 import ssm_scan, ssm_update
+
+    ops = to_dev(ref.case(107, 1, seqlen, 24, dstate, dtype=dtype))
+    assert (pieces(ops, False) > 1) == (seqlen > 100)
+    bad = dict(ops, A=ops["A"].clone())
+    bad["A"][5, 3] = float("nan")
+    outs = []
+    for o in (ops, bad):
+        o["A"].requires_grad_(True)
+        out, fin = ssm_scan(**o, dt_softplus=True, return_final_states=True)
+        (dA,) = torch.autograd.grad(out, [o["A"]], torch.ones_like(out))
+        state = torch.zeros(1, 24, dstate, device=DEV)
+        token = {k: v.detach() if v is not None else v for k, v in token_ops(o, 0).items()}
+        y = ssm_update(ssm_state=state, dt_softplus=True, **token)
+        y3 = ssm_update(ssm_state=state.clone(), dt_softplus=True, **{k: v.detach() if v is not None else v for k, v in
+                                                                      token_ops(o, slice(0, 3)).items()})
+        outs.append((out.detach(), fin.detach(), dA, state, y, y3))
+    for clean, got, axis in zip(*outs, (-1, None, None, None, -1, -1)):
+        where = torch.zeros_like(clean, dtype=torch.bool)
+        if axis == -1:
+            where[..., 5] = True
+        else:
+            where[..., 5, 3] = True
+        assert not clean.isnan().any()
+        if clean is outs[0][2]:  # the channel's other gradients pass through its output's sum alone
+            assert got[5, 3].isnan() and torch.equal(got[~where], clean[~where])
+        else:
+            assert torch.equal(got.isnan(), where) and torch.equal(got[~where], clean[~where])
