@@ -362,6 +362,15 @@ __device__ __forceinline__ SsmPlace ssm_place(const SsmParams& p) {
   return w;
 }
 
+// What leaves a piece of decay d and own result o that receives `carry`. A piece in which a sequence starts,
+// through which nothing passes, is marked by a negative decay: a decay itself may underflow to 0, after which a
+// state is still infinite or NaN if it was before, and overflow (A > 0), after which a zero is still zero.
+constexpr float kSsmCut = -1.0f;
+__device__ __forceinline__ float pass_piece(float d, float carry, float o) {
+  if (d < 0.0f || carry == 0.0f) return o;
+  return fmaf(d == 0.0f && isinf(carry) ? 1.0f : d, carry, o);
+}
+
 // What piece w.seg of the sequence receives, into h: of channels ch and ch + 1 the pairs of states that
 // start at n1 and n2. From the join kernel, or, with few pieces, by the same chain over the pieces before
 // (after) it, whose loads are independent of it.
@@ -392,8 +401,8 @@ __device__ __forceinline__ void piece_in(const SsmParams& p, const SsmPlace& w, 
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        h[c][m].x = d[c][m].x == 0.0f ? o[c][m].x : fmaf(d[c][m].x, h[c][m].x, o[c][m].x);
-        h[c][m].y = d[c][m].y == 0.0f ? o[c][m].y : fmaf(d[c][m].y, h[c][m].y, o[c][m].y);
+        h[c][m].x = pass_piece(d[c][m].x, h[c][m].x, o[c][m].x);
+        h[c][m].y = pass_piece(d[c][m].y, h[c][m].y, o[c][m].y);
       }
   }
 }

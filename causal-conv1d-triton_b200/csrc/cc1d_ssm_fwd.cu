@@ -43,8 +43,8 @@ struct ScanSmem {
 //
 // PASS kSsmForward is that. The other two prepare a sequence cut in pieces: kSsmPieceForward finds
 // the state that a piece leaves when it starts from zero, kSsmPieceBackward the gradient that it
-// passes back when it receives none, each with the piece's decay exp(A sum delta); launch_ssm_join
-// chains them. SEQ: packed rows (seq_idx).
+// passes back when it receives none, each with the piece's decay exp(A sum delta), or kSsmCut where a
+// sequence starts in it; launch_ssm_join or piece_in chains them. SEQ: packed rows (seq_idx).
 template <typename T, int NL, int PASS, bool SEQ>
 struct Scan {
   using S = ScanSmem<T, NL>;
@@ -330,7 +330,7 @@ struct Scan {
         const int64_t i = (piece + ch) * NP + n0;
         const float2 e0 = decay2<T>(fmul2(splat(sum_delta[c]), A2[c][0])), e1 = decay2<T>(fmul2(splat(sum_delta[c]), A2[c][1]));
         *reinterpret_cast<float4*>(p.seg_out + i) = s4;
-        *reinterpret_cast<float4*>(p.seg_decay + i) = cut ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(e0.x, e0.y, e1.x, e1.y);
+        *reinterpret_cast<float4*>(p.seg_decay + i) = cut ? make_float4(kSsmCut, kSsmCut, kSsmCut, kSsmCut) : make_float4(e0.x, e0.y, e1.x, e1.y);
       }
     }
   }
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(128) cc1d_ssm_join_kernel(const float* __restr
   for (int s = 1; s < segs - 1; ++s) {
     const float o = own[at + s * step], d = decay[at + s * step];
     in[at + s * step] = carry;
-    carry = d == 0.0f ? o : fmaf(d, carry, o);
+    carry = pass_piece(d, carry, o);
   }
   in[at + (segs - 1) * step] = carry;  // the last piece's own result is not needed and was not computed
 }

@@ -706,3 +706,74 @@ def test_nan_in_a_decay_rate(dtype, seqlen, dstate):
             assert got[5, 3].isnan() and torch.equal(got[~where], clean[~where])
         else:
             assert torch.equal(got.isnan(), where) and torch.equal(got[~where], clean[~where])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("seqlen", [40, 300, 700])  # one piece; pieces chained by themselves, and by a kernel
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("rate", [-20.0, -60.0])
+def test_states_stay_non_finite_across_pieces(dtype, seqlen, bad, rate):
+    """A state or gradient that is infinite or NaN stays so where a piece's decay underflows, and ends where a
+    sequence starts; the others have their usual bits. At a rate of -60 single steps underflow too, where an
+    infinity times 0 becomes a NaN."""
+    from causal_conv1d_b200 import ssm_scan
+
+    ops = to_dev(ref.case(109, 1, seqlen, 24, 16, dtype=dtype, init=True))
+    ops["A"][5, 3] = rate
+    ops["dt_bias"][:] = 0.0  # steps of about 0.7: 32 of them times 20 pass what 32 bits hold
+    n = pieces(ops, False)
+    assert n == 1 if seqlen == 40 else 2 < n <= 16 if seqlen == 300 else n > 16
+    dfin = torch.randn(1, 24, 16, device=DEV)
+    res = []
+    for first, last in ((ops["initial_states"], dfin), [t.index_put((torch.tensor(0), torch.tensor(5), torch.tensor(3)),
+                                                                    torch.tensor(bad, device=DEV)) for t in (ops["initial_states"], dfin)]):
+        h0 = first.clone().requires_grad_(True)
+        out, fin = ssm_scan(**dict(ops, initial_states=h0), dt_softplus=True, return_final_states=True)
+        (dh0,) = torch.autograd.grad(fin, h0, last)
+        res.append((fin.detach(), dh0))
+    for clean, got in zip(*res):
+        assert not got[0, 5, 3].isfinite()
+        if rate == -20.0:
+            assert torch.equal(got[0, 5, 3].nan_to_num(nan=5.0), torch.tensor(bad, device=DEV).nan_to_num(nan=5.0))
+        got[0, 5, 3] = clean[0, 5, 3]
+        assert clean.isfinite().all() and torch.equal(got, clean)
+    # Packed rows: the next sequence does not receive it.
+    seq = torch.zeros(1, seqlen, device=DEV, dtype=torch.int32)
+    seq[:, seqlen // 2:] = 1
+    packed = []
+    for first in (0.0, bad):
+        h0 = torch.zeros(1, 24, 16, device=DEV)
+        h0[0, 5, 3] = first
+        packed.append(ssm_scan(**dict(ops, initial_states=h0, seq_idx=seq), dt_softplus=True))
+    assert torch.equal(packed[1][:, seqlen // 2:], packed[0][:, seqlen // 2:]) and packed[0].isfinite().all()
+    assert not packed[1][0, :seqlen // 2, 5].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("seqlen", [300, 700])
+def test_nothing_grows_out_of_zero_across_pieces(dtype, seqlen):
+    """Growing states (A > 0) whose growth over a piece passes what 32 bits hold: no state before the last tokens,
+    no gradient behind the first ones."""
+    from causal_conv1d_b200 import ssm_scan
+
+    ops = to_dev(ref.case(113, 1, seqlen, 24, 16, dtype=dtype, z=False))
+    # Steps of about 0.7: 32 of them times 5 pass what 32 bits hold, three do not.
+    ops["A"], ops["dt_bias"] = 5.0 + ops["A"].abs() / 16, torch.zeros(24, device=DEV)
+    ops["x"][:, :-3] = 0.0
+    assert pieces(ops, False) > 1 and pieces(ops, True) > 1
+    mine = {k: v.clone().requires_grad_(True) if k in ("x", "dt", "B", "C") else v for k, v in ops.items()}
+    want = ref.wide(ops)
+    out = ssm_scan(**mine, dt_softplus=True)
+    wout, _ = ref.scan(**want, dt_softplus=True)
+    ref.assert_near(out, wout, seqlen, "out")
+    # Only the first three outputs count: the gradient ends there.
+    dout = torch.zeros_like(ops["x"])
+    dout[:, :3] = torch.randn(1, 3, 24, device=DEV).to(dtype)
+    for k in ("x", "dt", "B", "C"):
+        want[k] = want[k][:, :3].requires_grad_(True)
+    wout, _ = ref.scan(**want, dt_softplus=True)
+    got = torch.autograd.grad(out, [mine[k] for k in ("x", "dt", "B", "C")], dout)
+    exp = torch.autograd.grad(wout, [want[k] for k in ("x", "dt", "B", "C")], dout[:, :3].double())
+    for k, a, e in zip(("x", "dt", "B", "C"), got, exp):
+        ref.assert_near(a[:, :3], e, seqlen, "d" + k)
+        assert not a[:, 3:].any(), k
