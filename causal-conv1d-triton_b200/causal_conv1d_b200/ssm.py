@@ -14,7 +14,8 @@ in and out, `*_update` with slot indices for decoding. fp32/fp16/bf16 inputs; al
 every sum are fp32. The kernels (csrc/cc1d_ssm_*.cu, csrc/cc1d_slot_maps.cu) are behind the C ABI of
 include/causal_conv1d_b200.h and run on torch's current stream. The argument checks and the autograd
 Function are C++ (csrc/cc1d_torch_ssm.cpp): AssertionError for shapes and devices, TypeError for
-element types, CausalConv1dError for a failing library call.
+element types, NotImplementedError for forward-mode derivatives (tensors with a tangent), CausalConv1dError
+for a failing library call.
 """
 
 from __future__ import annotations

@@ -4,14 +4,15 @@
 // include/causal_conv1d_b200.h. All of it is C++ because it is all that a small call costs: a decode
 // step's kernel runs for 3 us, and the same checks written in Python took 17.
 //
-// Bad arguments raise AssertionError (shapes, devices) and TypeError (element types), a failing
-// library call the package's CausalConv1dError; inside the autograd Function, which runs on torch's
+// Bad arguments raise AssertionError (shapes, devices) and TypeError (element types), forward-mode tangents
+// NotImplementedError, a failing library call the package's CausalConv1dError; inside the autograd Function, which runs on torch's
 // own threads, it is a RuntimeError.
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <initializer_list>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -115,6 +116,17 @@ void check_operands(const at::Tensor& x, const at::Tensor& dt, const at::Tensor&
   for (const Opt* t : {&D, &dt_bias})
     if (t->has_value()) floating(**t);
   need(x.is_cuda(), "x must be on a CUDA device");
+}
+
+// Forward-mode derivatives: the kernels have none, and tensors that carry a tangent (torch.autograd.forward_ad)
+// would come out without one, which reads as a derivative of zero.
+void refuse_tangents(std::initializer_list<const at::Tensor*> given, std::initializer_list<const Opt*> optional) {
+  auto check = [](const at::Tensor& t) {
+    if (t._fw_grad(0).defined()) raise(PyExc_NotImplementedError, "the state-space operators have no forward-mode derivatives");
+  };
+  for (const at::Tensor* t : given) check(*t);
+  for (const Opt* t : optional)
+    if (t->has_value()) check(**t);
 }
 
 void check_cache(const at::Tensor& state, const at::Tensor& x, int64_t dstate) {
@@ -237,6 +249,7 @@ struct SsmFn : public torch::autograd::Function<SsmFn> {
 py::object ssm_scan(const at::Tensor& x0, const at::Tensor& dt0, const at::Tensor& A0, const at::Tensor& B0,
                     const at::Tensor& C0, const Opt& D0, const Opt& z0, const Opt& dt_bias0, bool softplus,
                     const Opt& seq_idx0, const Opt& init0, bool return_final, const Opt& state, const Opt& indices0) {
+  refuse_tangents({&x0, &dt0, &A0, &B0, &C0}, {&D0, &z0, &dt_bias0, &init0, &state});
   need(x0.dim() == 3, "x must be (batch, seqlen, dim)");
   check_operands(x0, dt0, A0, B0, C0, D0, z0, dt_bias0, false);
   const int64_t batch = x0.size(0), seqlen = x0.size(1), dim = x0.size(2), dstate = A0.size(1);
@@ -286,6 +299,7 @@ py::object ssm_scan(const at::Tensor& x0, const at::Tensor& dt0, const at::Tenso
 at::Tensor ssm_update(const at::Tensor& x0, const at::Tensor& state, const at::Tensor& dt0, const at::Tensor& A0,
                       const at::Tensor& B0, const at::Tensor& C0, const Opt& D0, const Opt& z0, const Opt& dt_bias0,
                       bool softplus, const Opt& indices0) {
+  refuse_tangents({&x0, &state, &dt0, &A0, &B0, &C0}, {&D0, &z0, &dt_bias0});
   need(x0.dim() == 2 || x0.dim() == 3, "x must be (batch, dim) or (batch, seqlen, dim)");
   const bool one = x0.dim() == 2;
   check_operands(x0, dt0, A0, B0, C0, D0, z0, dt_bias0, one);

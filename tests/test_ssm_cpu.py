@@ -132,3 +132,21 @@ def test_c_entry_points_refuse_unaligned_scratch():
         assert n.lib.cc1d_ssm_fwd(ctypes.byref(q), 4096, None, kept, None, 0, 0, None, 0, workspace, 1 << 30, None) == n.CC1D_ERR_INVALID
         assert n.lib.cc1d_ssm_bwd(ctypes.byref(q), ctypes.byref(dout), kept, None, ctypes.byref(grads), workspace, 1 << 30,
                                   None) == n.CC1D_ERR_INVALID
+
+
+@pytest.mark.parametrize("name", ["x", "dt", "A", "B", "C", "D", "z", "dt_bias", "initial_states", "ssm_state"])
+def test_forward_mode_is_refused(name):
+    """A tangent would be lost without a word (nothing requires grad in forward mode)."""
+    import torch.autograd.forward_ad as fwad
+
+    from causal_conv1d_b200 import ssm_scan, ssm_update
+
+    ops = operands(initial_states=torch.zeros(2, 6, 4))
+    token = {k: v[:, 0] if k in ("x", "dt", "B", "C", "z") else v for k, v in ops.items() if k not in ("seq_idx", "initial_states")}
+    token["ssm_state"] = torch.zeros(2, 6, 4)
+    with fwad.dual_level():
+        for fn, args in ((ssm_scan, ops), (ssm_update, token)):
+            if name in args:
+                dual = fwad.make_dual(args[name], torch.ones_like(args[name]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    fn(**{**args, name: dual})
