@@ -147,6 +147,12 @@ at::Tensor int32s(const at::Tensor& t, const at::Tensor& x) {
   return (t.scalar_type() == at::kInt && t.device() == x.device() ? t : t.to(x.device(), at::kInt)).contiguous();
 }
 
+// The kernels write a state through its address: autograd learns of it by the version, and then refuses a
+// backward over a graph that saved the values before. Tensors made under inference mode have no version.
+void written_in_place(const at::Tensor& state) {
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor floats(const at::Tensor& like, int64_t bytes) { return empty({std::max<int64_t>(1, bytes / 4)}, at::kFloat, like); }
 
 // h after the last token of an input without tokens.
@@ -292,6 +298,7 @@ py::object ssm_scan(const at::Tensor& x0, const at::Tensor& dt0, const at::Tenso
   auto [rc, out, final, kept] =
       ssm_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, seq_idx, init, return_final, false, state, indices);
   check(rc, "ssm_scan");
+  if (state.has_value()) written_in_place(*state);
   if (return_final) return py::make_tuple(out, *final);
   return py::cast(out);
 }
@@ -319,6 +326,7 @@ at::Tensor ssm_update(const at::Tensor& x0, const at::Tensor& state, const at::T
   const cc1d_ssm_problem q = problem(x, dt, A, B, C, D, z, dt_bias, softplus, c10::nullopt, c10::nullopt, one);
   check(cc1d_ssm_update(&q, state.data_ptr(), dtype_code(state), state.size(0), ints(indices), out.data_ptr(), stream_of(x)),
         "ssm_update");
+  written_in_place(state);
   return out;
 }
 

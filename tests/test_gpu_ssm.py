@@ -777,3 +777,27 @@ def test_nothing_grows_out_of_zero_across_pieces(dtype, seqlen):
     for k, a, e in zip(("x", "dt", "B", "C"), got, exp):
         ref.assert_near(a[:, :3], e, seqlen, "d" + k)
         assert not a[:, 3:].any(), k
+
+
+def test_autograd_sees_states_written_in_place():
+    """A graph that saved a state before an operator wrote to it refuses its backward, as after any in-place
+    operation; a state made under inference mode, which has no version, can still be written."""
+    from causal_conv1d_b200 import ssm_scan, ssm_update
+
+    ops = to_dev(ref.case(127, 1, 20, 24, 16, lengths=[[8, 12]]))
+    slots = torch.tensor([0, 1], device=DEV)
+    token = {k: v.expand(2, *v.shape[1:]) if k in ("x", "dt", "B", "C", "z") else v for k, v in token_ops(ops, 0).items()}
+    writes = (lambda s: ssm_update(ssm_state=s, ssm_state_indices=slots, **token),
+              lambda s: ssm_scan(**ops, ssm_state=s, ssm_state_indices=slots[None]))
+    for write in writes:
+        state, w = torch.ones(2, 24, 16, device=DEV), torch.ones(16, device=DEV, requires_grad=True)
+        y = (state * w).sum()
+        with torch.no_grad():
+            write(state)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            y.backward()
+        with torch.inference_mode():
+            made = torch.ones(2, 24, 16, device=DEV)
+            write(made)
+        with torch.no_grad():
+            write(made)
