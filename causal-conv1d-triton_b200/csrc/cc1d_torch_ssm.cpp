@@ -143,6 +143,9 @@ at::Tensor vector(const at::Tensor& t) { return (dtype_code(t) < 0 ? t.to(at::kF
 Opt vector(const Opt& t) { return t.has_value() ? Opt(vector(*t)) : t; }
 at::Tensor rows(const at::Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 Opt rows(const Opt& t) { return t.has_value() ? Opt(rows(*t)) : t; }
+void need_integer(const at::Tensor& t, const char* what) {
+  if (t.is_floating_point() || t.is_complex()) raise(PyExc_TypeError, std::string(what) + " must be integer, got " + name(t));
+}
 at::Tensor int32s(const at::Tensor& t, const at::Tensor& x) {
   return (t.scalar_type() == at::kInt && t.device() == x.device() ? t : t.to(x.device(), at::kInt)).contiguous();
 }
@@ -264,6 +267,7 @@ py::object ssm_scan(const at::Tensor& x0, const at::Tensor& dt0, const at::Tenso
     need(!return_final, "cannot return final states if seq_idx is not None");
     need(seq_idx0->dim() == 2 && seq_idx0->size(0) == batch && seq_idx0->size(1) == seqlen, "seq_idx must be (batch, seqlen)");
     need(seq_idx0->device() == x0.device(), "all operands must be on x's device");
+    need_integer(*seq_idx0, "seq_idx");
     seq_idx = int32s(*seq_idx0, x0);
   }
   if (init0.has_value()) {
@@ -278,6 +282,7 @@ py::object ssm_scan(const at::Tensor& x0, const at::Tensor& dt0, const at::Tenso
     check_cache(*state, x0, dstate);
     need(indices0->dim() == 1 ? batch == 1 : indices0->dim() == 2 && indices0->size(0) == batch,
          "ssm_state_indices must be (batch, n_seqs)");
+    need_integer(*indices0, "ssm_state_indices");
     indices = int32s(*indices0, x0);
   } else {
     need(!indices0.has_value(), "ssm_state_indices requires ssm_state");
@@ -314,6 +319,7 @@ at::Tensor ssm_update(const at::Tensor& x0, const at::Tensor& state, const at::T
   Opt indices;
   if (indices0.has_value()) {
     need(indices0->dim() == 1 && indices0->size(0) == x0.size(0), "ssm_state_indices must be (batch,)");
+    need_integer(*indices0, "ssm_state_indices");
     indices = int32s(*indices0, x0);
   } else {
     need(state.size(0) >= x0.size(0), "ssm_state has fewer slots than x has rows");
@@ -345,7 +351,7 @@ py::tuple slot_maps(const at::Tensor& lengths0, int64_t seqlen, int64_t width, c
   need(slots0.has_value() || !free0.has_value(), "free_slots requires slots");
   const int64_t n = lengths0.size(0);
   auto integer = [&](const at::Tensor& t, const char* what) {
-    if (t.is_floating_point() || t.is_complex()) raise(PyExc_TypeError, std::string(what) + " must be integer, got " + name(t));
+    need_integer(t, what);
     if (t.dim() != 1) raise(PyExc_AssertionError, std::string(what) + " must be 1-D");
     if (t.device() != lengths0.device()) raise(PyExc_AssertionError, std::string(what) + " must be on the device of lengths");
   };

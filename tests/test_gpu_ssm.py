@@ -801,3 +801,20 @@ def test_autograd_sees_states_written_in_place():
             write(made)
         with torch.no_grad():
             write(made)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, torch.float64, torch.complex64])
+def test_ids_and_slots_are_integers(dtype):
+    from causal_conv1d_b200 import ssm_scan, ssm_update
+
+    ops = to_dev(ref.case(131, 2, 6, 8, 4, lengths=[[2, 4], [6]]))
+    state, slots = torch.zeros(4, 8, 4, device=DEV), torch.tensor([[0, 1], [2, -1]], device=DEV)
+    with pytest.raises(TypeError, match="seq_idx must be integer"):
+        ssm_scan(**dict(ops, seq_idx=ops["seq_idx"].to(dtype)))
+    with pytest.raises(TypeError, match="ssm_state_indices must be integer"):
+        ssm_scan(**ops, ssm_state=state, ssm_state_indices=slots.to(dtype))
+    with pytest.raises(TypeError, match="ssm_state_indices must be integer"):
+        ssm_update(ssm_state=state, ssm_state_indices=slots[:, 0].to(dtype), **token_ops(ops, 0))
+    assert not state.any()
+    for kind in (torch.int64, torch.int32, torch.int16):
+        ssm_update(ssm_state=state, ssm_state_indices=slots[:, 0].to(kind), **token_ops(ops, 0))
