@@ -365,6 +365,7 @@ __device__ __forceinline__ SsmPlace ssm_place(const SsmParams& p) {
 // What leaves a piece of decay d and own result o that receives `carry`. A piece in which a sequence starts,
 // through which nothing passes, is marked by a negative decay: a decay itself may underflow to 0, after which a
 // state is still infinite or NaN if it was before, and overflow (A > 0), after which a zero is still zero.
+// fmaf(d, carry, o) alone is right unless it gives a NaN.
 constexpr float kSsmCut = -1.0f;
 __device__ __forceinline__ float pass_piece(float d, float carry, float o) {
   if (d < 0.0f || carry == 0.0f) return o;
@@ -401,9 +402,31 @@ __device__ __forceinline__ void piece_in(const SsmParams& p, const SsmPlace& w, 
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        h[c][m].x = pass_piece(d[c][m].x, h[c][m].x, o[c][m].x);
-        h[c][m].y = pass_piece(d[c][m].y, h[c][m].y, o[c][m].y);
+        h[c][m].x = d[c][m].x < 0.0f ? o[c][m].x : fmaf(d[c][m].x, h[c][m].x, o[c][m].x);
+        h[c][m].y = d[c][m].y < 0.0f ? o[c][m].y : fmaf(d[c][m].y, h[c][m].y, o[c][m].y);
       }
+  }
+  // A NaN may be one of 0 times infinity: then the chain once more, by pass_piece (whose tests at every step
+  // cost a chain of 15 pieces 2 us, and its branches, which keep loads from being issued early, 7).
+  bool nan = false;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) nan = nan || isnan(h[c][m].x) || isnan(h[c][m].y);
+  if (nan) {
+    read(p.seg_out, from, h);
+#pragma unroll 1
+    for (int i = 1; i < n; ++i) {
+      float2 o[2][2], d[2][2];
+      read(p.seg_out, from + i * step, o), read(p.seg_decay, from + i * step, d);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          h[c][m].x = pass_piece(d[c][m].x, h[c][m].x, o[c][m].x);
+          h[c][m].y = pass_piece(d[c][m].y, h[c][m].y, o[c][m].y);
+        }
+    }
   }
 }
 
