@@ -268,7 +268,7 @@ struct Bwd {
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          a[c][m] = decay2<T>(fmul2(splat(d[c]), A2[c][m]));
+          a[c][m] = decay2<T>(splat(d[c]), A2[c][m]);
           h[c][m] = ffma2(a[c][m], h[c][m], fmul2(splat(u[c]), B[m]));
         }
     };

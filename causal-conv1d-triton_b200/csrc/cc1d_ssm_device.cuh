@@ -13,8 +13,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
 
-// 2^x, one MUFU operation. Measured against 64 bits over -16 < x < 0 it is at most 1.4e-7 off, and 5e-8
-// low on average (1e-8 at x = -2^-10).
+// 2^x, one MUFU operation. Measured against 64 bits over -16 < x < 0 it is at most 1.4e-7 off, and low on
+// average: 5e-8 for x < -1, about 2e-8 between -2^-1 and -2^-8, 6e-9 from -2^-10 on.
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -22,14 +22,16 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 __device__ __forceinline__ float2 exp2_approx2(float2 x) { return make_float2(exp2_approx(x.x), exp2_approx(x.y)); }
 
-// 2^x = 2^i 2^f with i the nearest integer (found by adding and taking off 1.5 2^23) and 2^f, |f| <= 1/2, by
-// its Taylor polynomial of degree 6 (ln2^k / k!, below 2e-7 off at |f| = 1/2 and exact to rounding for small
-// f). Arguments below -126 give 2^-126, above 127.5 infinity. A NaN gives a NaN: it passes the limits, and the
-// power of two, which means nothing then, is multiplied and not added to the exponent's bits.
+// x limited to [lo, hi]; a NaN stays one.
 __device__ __forceinline__ float within(float x, float lo, float hi) {
   asm("max.NaN.f32 %0, %0, %1;\n\tmin.NaN.f32 %0, %0, %2;" : "+f"(x) : "f"(lo), "f"(hi));
   return x;
 }
+
+// 2^x = 2^i 2^f with i the nearest integer (found by adding and taking off 1.5 2^23) and 2^f, |f| <= 1/2, by
+// its Taylor polynomial of degree 6 (ln2^k / k!, below 2e-7 off at |f| = 1/2 and exact to rounding for small
+// f). Arguments below -126 give 2^-126, above 127.5 infinity. A NaN gives a NaN: it passes the limits, and the
+// power of two, which means nothing then, is multiplied and not added to the exponent's bits.
 __device__ __forceinline__ float2 exp2_exact2(float2 x) {
   x = make_float2(within(x.x, -126.0f, 128.0f), within(x.y, -126.0f, 128.0f));
   const float2 t = fadd2(x, splat(12582912.0f)), f = fadd2(x, fmul2(fadd2(t, splat(-12582912.0f)), splat(-1.0f)));
@@ -44,15 +46,18 @@ __device__ __forceinline__ float2 exp2_exact2(float2 x) {
 }
 
 // The decay of a step, for operands of type T. A one-sided error adds up over as many tokens as a state
-// remembers: with the MUFU's, dA of 2048 tokens comes out 2e-6 off in norm and states 6e-7 (with the
-// polynomial 4e-7 and 1.5e-7). That is far below what 16-bit operands carry, and twice the speed; operands
-// in 32 bits take the polynomial.
+// remembers. The MUFU's is met by an addend to the exponent, which comes free with the product: with 2e-8 the mean
+// is below 1.2e-8 either way for |x| < 2^-2 (a multiply-add rounds small arguments finely enough to keep it; 2^2e-8
+// itself is 1, so that a step of 0 changes nothing). 3e-8 would leave less at 2^-7 and twice as much at 2^-10, where the
+// memory is longest. dA of 4 x 2048 tokens is then 8.3e-7 off in norm (1.8e-6 without the addend; the same sums in
+// 32 bits with a library exponential 9.8e-7), at the same speed. Operands in 32 bits take the polynomial, whose
+// error has no side.
+constexpr float kExp2Addend = 2e-8f;
 template <typename T>
-__device__ __forceinline__ float2 decay2(float2 x) {
-  if constexpr (sizeof(T) == 4) return exp2_exact2(x);
-  else return exp2_approx2(x);
+__device__ __forceinline__ float2 decay2(float2 delta, float2 A2) {
+  if constexpr (sizeof(T) == 4) return exp2_exact2(fmul2(delta, A2));
+  else return exp2_approx2(ffma2(delta, A2, splat(kExp2Addend)));
 }
-
 
 // log(1 + exp(v)) = max(v, 0) + log1p(w) with w = exp(-|v|) in (0, 1]. log1p(w) = 2 atanh(s) with
 // s = w / (2 + w) <= 1/3, whose series 2 s (1 + s^2/3 + s^4/5 + ...) after seven terms is 3e-8 off

@@ -246,7 +246,7 @@ struct Scan {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m) a[k & 1][c][m] = decay2<T>(fmul2(splat(d[c]), A2[c][m]));
+            for (int m = 0; m < 2; ++m) a[k & 1][c][m] = decay2<T>(splat(d[c]), A2[c][m]);
             if constexpr (!FWD) sum_delta[c] += d[c];
           }
         };
@@ -328,7 +328,7 @@ struct Scan {
         }
       } else {
         const int64_t i = (piece + ch) * NP + n0;
-        const float2 e0 = decay2<T>(fmul2(splat(sum_delta[c]), A2[c][0])), e1 = decay2<T>(fmul2(splat(sum_delta[c]), A2[c][1]));
+        const float2 e0 = decay2<T>(splat(sum_delta[c]), A2[c][0]), e1 = decay2<T>(splat(sum_delta[c]), A2[c][1]);
         *reinterpret_cast<float4*>(p.seg_out + i) = s4;
         *reinterpret_cast<float4*>(p.seg_decay + i) = cut ? make_float4(kSsmCut, kSsmCut, kSsmCut, kSsmCut) : make_float4(e0.x, e0.y, e1.x, e1.y);
       }

@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kStep, 1024 / kStep) cc1d_ssm_step_kernel(cons
       const float4 b = unpack4(B[r]), c = unpack4(C[r]);
       float2 h[2];
       load_vec<ST, 4>(reinterpret_cast<const ST*>(staged) + ((q * kRows + r) * kStep + threadIdx.x) * 4, h);
-      const float2 a0 = decay2<T>(fmul2(d, A2[0])), a1 = decay2<T>(fmul2(d, A2[1]));
+      const float2 a0 = decay2<T>(d, A2[0]), a1 = decay2<T>(d, A2[1]);
       h[0] = ffma2(a0, h[0], fmul2(v, make_float2(b.x, b.y)));
       h[1] = ffma2(a1, h[1], fmul2(v, make_float2(b.z, b.w)));
       const float2 s = ffma2(h[1], make_float2(c.z, c.w), fmul2(h[0], make_float2(c.x, c.y)));
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(256, 2) cc1d_ssm_update_kernel(const __grid_co
       const int from = lead + ((r >> 1) | ((r & 1) << 1));
       const float2 d = splat(__shfl_sync(0xffffffffu, delta, from)), v = splat(__shfl_sync(0xffffffffu, u, from));
       const float4 b = unpack4(B[r]), c = unpack4(C[r]);
-      const float2 a0 = decay2<T>(fmul2(d, A2[0])), a1 = decay2<T>(fmul2(d, A2[1]));
+      const float2 a0 = decay2<T>(d, A2[0]), a1 = decay2<T>(d, A2[1]);
       h[r][0] = ffma2(a0, h[r][0], fmul2(v, make_float2(b.x, b.y)));
       h[r][1] = ffma2(a1, h[r][1], fmul2(v, make_float2(b.z, b.w)));
       const float2 s = ffma2(h[r][1], make_float2(c.z, c.w), fmul2(h[r][0], make_float2(c.x, c.y)));
