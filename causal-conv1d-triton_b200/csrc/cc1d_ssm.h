@@ -70,6 +70,7 @@ struct SsmUpdateParams {
   void* out;               // (batch, seqlen, dim) contiguous
   int batch, seqlen, dim, dstate, group_dim;
   int softplus;
+  int sms;                 // of the device
   int blocks;              // set by the launcher: CTAs over the channels
 };
 

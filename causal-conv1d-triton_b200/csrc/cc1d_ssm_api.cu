@@ -264,6 +264,7 @@ int cc1d_ssm_update(const cc1d_ssm_problem* q, void* state, int state_dtype, int
   p.batch = static_cast<int>(q->batch), p.seqlen = static_cast<int>(q->seqlen), p.dim = static_cast<int>(q->dim);
   p.dstate = static_cast<int>(q->dstate), p.group_dim = static_cast<int>(q->dim / q->groups);
   p.softplus = q->dt_softplus != 0;
+  CC1D_TRY(device_sms(&p.sms));
   if (cdiv(q->batch * q->dim * ssm_lanes(p.dstate), 256) > kMaxInt) return CC1D_ERR_INVALID;
   return done(launch_ssm_update(p, static_cast<cudaStream_t>(stream)));
 }
