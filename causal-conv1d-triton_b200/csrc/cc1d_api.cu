@@ -603,7 +603,7 @@ const char* cc1d_error_string(int code) {
     case CC1D_OK: return "success";
     case CC1D_ERR_INVALID: return "invalid argument (size, stride, dtype code or missing pointer)";
     case CC1D_ERR_UNSUPPORTED: return "unsupported size (the largest width is 256, the largest state 64 per channel)";
-    case CC1D_ERR_WORKSPACE: return "workspace smaller than cc1d_bwd_workspace_bytes()";
+    case CC1D_ERR_WORKSPACE: return "workspace smaller than the entry point's *_workspace_bytes() says";
     case CC1D_ERR_CUDA: return "CUDA call failed (see cc1d_last_cuda_error())";
     case CC1D_ERR_SCRATCH_LIMIT:
       return "backward needs more scratch than cc1d_bwd_noalloc's fixed 8 MiB buffer; call cc1d_bwd with a workspace";

@@ -40,7 +40,7 @@ enum {
   CC1D_OK = 0,
   CC1D_ERR_INVALID = 1,     /* bad size, stride, dtype code or missing required pointer */
   CC1D_ERR_UNSUPPORTED = 2, /* width above the largest supported (256), or state above 64 */
-  CC1D_ERR_WORKSPACE = 3,   /* workspace smaller than cc1d_bwd_workspace_bytes() */
+  CC1D_ERR_WORKSPACE = 3,   /* workspace smaller than the entry point's *_workspace_bytes() says */
   CC1D_ERR_CUDA = 4,        /* a CUDA runtime/driver call failed; see cc1d_last_cuda_error() */
   CC1D_ERR_SCRATCH_LIMIT = 5, /* cc1d_bwd_noalloc: problem needs more than its fixed scratch */
   CC1D_ERR_LAYOUT = 6         /* cc1d_bwd_split: pieces or dx strides outside its fast path */

@@ -150,3 +150,10 @@ def test_forward_mode_is_refused(name):
                 dual = fwad.make_dual(args[name], torch.ones_like(args[name]))
                 with pytest.raises(NotImplementedError, match="forward-mode"):
                     fn(**{**args, name: dual})
+
+
+def test_error_texts_name_no_other_entry_point():
+    from causal_conv1d_b200 import _native as n
+
+    text = n.lib.cc1d_error_string(n.CC1D_ERR_WORKSPACE).decode()
+    assert "workspace" in text and "cc1d_bwd" not in text
