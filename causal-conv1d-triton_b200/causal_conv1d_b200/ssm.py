@@ -59,7 +59,12 @@ def ssm_scan(
     return_final_states: also return h after the last token, fp32; supports grad
     ssm_state, ssm_state_indices: with seq_idx, a (n_slots, dim, dstate) buffer that gets each
         packed sequence's last h, at slot ssm_state_indices[b, id] ((batch, n_seqs), or (n_seqs,)
-        for one row); ids without an entry and negative slots are skipped. Not differentiable
+        for one row); ids without an entry and negative slots are skipped. The buffer is written and
+        not read: every sequence but a row's first starts from zero, also where its slot holds a state,
+        so a request that continues does not belong in a packed row (give it a row of its own with
+        initial_states=ssm_state[slot], or take its tokens through ssm_update). An id must not come
+        back later in its row and no two sequences may share a slot: which one's h stays is not
+        defined. Not differentiable
 
     Returns out of x's shape and dtype, or (out, final_states). Every floating input but ssm_state
     gets a gradient; the gradients are deterministic, and not differentiable themselves. The forward keeps h before every 16th token

@@ -251,7 +251,8 @@ int64_t cc1d_ssm_workspace_bytes(int64_t batch, int64_t seqlen, int64_t dim, int
  *   kept_states   cc1d_ssm_kept_bytes() bytes, or NULL when no backward follows
  *   packed_state  (n_slots, dim, dstate) or NULL: with seq_idx, h after the last token of sequence id i of
  *                 row b goes to slot packed_slots[b * packed_slots_n + i]; ids at or above packed_slots_n
- *                 and slots outside [0, n_slots) are skipped
+ *                 and slots outside [0, n_slots) are skipped. Written only, not read. An id must not come back
+ *                 later in its row and no two sequences may share a slot: which one's h stays is not defined
  *   workspace     at least cc1d_ssm_workspace_bytes(..., x_dtype, 0) bytes
  */
 int cc1d_ssm_fwd(const cc1d_ssm_problem* problem, void* out, float* final_states, float* kept_states,

@@ -843,3 +843,29 @@ def test_decays_have_no_side(dtype, mean):
     want = torch.exp(A.double() * dt.double().sum(1)[..., None])
     off = (fin.double() / want - 1).mean((0, 1)) / T
     assert (off.abs() <= mean).all(), off.tolist()
+
+
+def test_packed_rows_hold_new_requests():
+    """What a slot held before does not enter a packed scan; the documented ways to continue a request do."""
+    from causal_conv1d_b200 import ssm_scan, ssm_update
+
+    ops = to_dev(ref.case(139, 1, 30, 24, 16, lengths=[[12, 18]]))
+    slots = torch.tensor([2, 0], device=DEV)
+    states = []
+    for held in (0.0, 3.0):
+        states.append(torch.full((4, 24, 16), held, device=DEV))
+        with torch.no_grad():
+            ssm_scan(**ops, dt_softplus=True, ssm_state=states[-1], ssm_state_indices=slots)
+    assert torch.equal(states[0][slots], states[1][slots]) and (states[1][[1, 3]] == 3).all()
+    # The first request once more, as the continuation of what its slot holds now.
+    first = {k: v[:, :12] if k in ("x", "dt", "B", "C", "z") else v for k, v in ops.items() if k != "seq_idx"}
+    whole = dict(ref.wide(ops), seq_idx=None)
+    for k in ("x", "dt", "B", "C", "z"):
+        whole[k] = torch.cat([whole[k][:, :12]] * 2, 1)
+    wout, wh = ref.scan(**whole, dt_softplus=True)
+    out, fin = ssm_scan(**dict(first, initial_states=states[0][2:3]), dt_softplus=True, return_final_states=True)
+    ref.assert_near(out, wout[:, 12:], 24)
+    ref.assert_near(fin, wh[:, -1], 24)
+    first.pop("initial_states")
+    assert torch.equal(ssm_update(ssm_state=states[0], dt_softplus=True, ssm_state_indices=slots[:1], **first), out)
+    assert torch.equal(states[0][2:3], fin)
