@@ -128,10 +128,14 @@ def slot_maps_from_lengths(
     seqlen: tokens of the packed row; what the lengths leave over is padding, and requests are cut at it
     width: of the convolution whose state rows `tail_rows` gives
     slots: (n,) state slot of each request, negative for none yet; a request with tokens and no slot
-        takes the next of free_slots, in request order (-1 once they are used up: n_taken tells)
+        takes the next of free_slots, in request order (-1 once they are used up: n_taken tells). It
+        takes it by its length, also where the cut at seqlen leaves none of its tokens in the row: no
+        scan then writes the slot, which still holds its last owner's state
     past_lengths: (n,) tokens that each request had before this step
 
     seq_idx goes to causal_conv1d_fn and ssm_scan, slots to ssm_scan(ssm_state_indices=) and the
-    updates, tail_rows picks the convolution's states out of its input.
+    updates, tail_rows picks the convolution's states out of its input. causal_conv1d_fn and ssm_scan
+    start every request of a packed row from zero: a row for them holds new requests alone, and a request
+    with past_lengths > 0 continues through the updates or through initial_states in a row of its own.
     """
     return SlotMaps._make(tex.slot_maps(lengths, seqlen, width, slots, free_slots, past_lengths))

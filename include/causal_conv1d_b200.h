@@ -298,7 +298,8 @@ int cc1d_ssm_update(const cc1d_ssm_problem* problem, void* state, int state_dtyp
  *   tail_rows     (n, width - 1) out: the rows of each request's last width - 1 tokens, what a convolution
  *                 of that width keeps; -1 for those before the request's first token
  *   slots_out     (n) out, with slots: the slot of each request; a request with tokens and no slot takes the
- *                 next of free_slots in request order (-1 once they are used up)
+ *                 next of free_slots in request order (-1 once they are used up), by its length, also where
+ *                 none of its tokens is left before seqlen
  *   n_taken       (1) out: how many requests needed a new slot
  */
 int cc1d_slot_maps(const int32_t* lengths, int64_t n, int64_t seqlen, int64_t width, const int32_t* past_lengths,

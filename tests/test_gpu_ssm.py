@@ -869,3 +869,17 @@ def test_packed_rows_hold_new_requests():
     first.pop("initial_states")
     assert torch.equal(ssm_update(ssm_state=states[0], dt_softplus=True, ssm_state_indices=slots[:1], **first), out)
     assert torch.equal(states[0][2:3], fin)
+
+
+def test_requests_cut_off_take_their_slots():
+    """By their length: the row ends before the last two, whose slots no scan writes."""
+    from causal_conv1d_b200 import slot_maps_from_lengths, ssm_scan
+
+    maps = slot_maps_from_lengths(torch.tensor([6, 9, 4, 0, 2], device=DEV), 10, slots=torch.full((5,), -1, device=DEV),
+                                  free_slots=torch.arange(7, device=DEV))
+    assert maps.slots.tolist() == [0, 1, 2, -1, 3] and maps.n_taken.tolist() == [4]
+    assert maps.cu_seqlens.tolist() == [0, 6, 10, 10, 10, 10]
+    ops = to_dev(ref.case(149, 1, 10, 8, 4))
+    state = torch.full((7, 8, 4), 3.0, device=DEV)
+    ssm_scan(**dict(ops, seq_idx=maps.seq_idx), dt_softplus=True, ssm_state=state, ssm_state_indices=maps.slots)
+    assert (state[2:] == 3).all() and not (state[:2] == 3).any()
