@@ -883,3 +883,130 @@ def test_requests_cut_off_take_their_slots():
     state = torch.full((7, 8, 4), 3.0, device=DEV)
     ssm_scan(**dict(ops, seq_idx=maps.seq_idx), dt_softplus=True, ssm_state=state, ssm_state_indices=maps.slots)
     assert (state[2:] == 3).all() and not (state[:2] == 3).any()
+
+
+def check_norms(ops, slots=None):
+    """Like check_scan, and what comes out in 32 bits also as a whole: within 1e-5 of the 64-bit form in norm.
+
+    A state is carried by decays that are off by 2e-7 each way (exponential, argument, step size), or, over a piece
+    of L tokens, by one decay of a sum of L steps, whose argument of size 16 or less (beyond, nothing is left of
+    the state) is off by 16 x 2^-24 for its own rounding and as much again for the sum's: 2e-6. A state remembers about
+    1/|log a| tokens, and in steps of 0.05 the slowest of them forgets within 20: 20 x 2e-7 + 2e-6 = 6e-6, and the
+    gradients, sums of such products without a common sign, stay below that too."""
+    from causal_conv1d_b200 import ssm_scan
+
+    g = torch.Generator().manual_seed(11)
+    dout = torch.randn(ops["x"].shape, generator=g).to(ops["x"].dtype).to(DEV)
+    mine, want = to_dev(ops), ref.wide(to_dev(ops))
+    names = [k for k in GRADS if ops[k] is not None]
+    final = ops["seq_idx"] is None
+    for d in (mine, want):
+        for k in names:
+            d[k] = d[k].detach().clone().requires_grad_(True)
+    res = ssm_scan(**mine, dt_softplus=True, return_final_states=final)
+    wout, wh = ref.scan(**want, dt_softplus=True)
+    got, exp = {}, {}
+    got["out"], exp["out"] = (res[0] if final else res), wout
+    if final:
+        got["final"], exp["final"] = res[1], wh[:, -1]
+    for d, o, w in ((got, mine, dout), (exp, want, dout.double())):
+        d.update(zip(names, torch.autograd.grad(d["out"], [o[k] for k in names], w)))
+    for k, a in got.items():
+        ref.assert_near(a, exp[k], ops["x"].shape[1], k)
+        if a.dtype == F32:
+            off = ((a.double() - exp[k]).norm() / exp[k].norm()).item()
+            assert off <= 1e-5, f"{k}: {off:.3g} off in norm"
+    return wh
+
+
+@pytest.mark.parametrize("batch, seqlen, dim, dstate, groups, dtype, kw, forward, backward", [
+    # Pieces chained by themselves, of 2 tiles and of 4 to 16, through which the buffers come round again.
+    (1, 300, 200, 16, 0, BF16, {}, 10, 10),
+    (2, 1024, 512, 16, 0, F16, dict(init=True), 16, 16),
+    (2, 1024, 512, 16, 0, F32, {}, 16, 8),
+    (1, 1000, 510, 40, 2, F32, dict(init=True), 8, 4),
+    (2, 1000, 1024, 24, 0, BF16, {}, 4, 16),
+    # By themselves forward and by the join kernel backward; by the join kernel, 6 tiles each.
+    (2, 700, 512, 24, 0, BF16, dict(init=True), 8, 22),
+    (1, 3000, 512, 16, 0, BF16, {}, 32, 32),
+    # Packed rows: sequences inside a piece, over several, from one's last token to the next one's first.
+    (2, 1024, 512, 16, 0, BF16, dict(init=True, lengths=[[10, 500, -2, 1, 319, 64, 128], [1024]]), 16, 16),
+    (3, 1021, 516, 12, 3, F32, dict(init=True, lengths=[[1021], [63, 1, 64, 700, -193], [-64, 957]]), 16, 16),
+    (1, 3000, 512, 16, 0, F16, dict(lengths=[[96, 95, 1, 1000, 1, 7, -100, 1700]]), 32, 32),
+])
+def test_pieces_of_every_plan(batch, seqlen, dim, dstate, groups, dtype, kw, forward, backward):
+    ops = ref.case(seqlen + dim, batch, seqlen, dim, dstate, groups, dtype, **kw)
+    assert (pieces(ops, False), pieces(ops, True)) == (forward, backward)
+    check_norms(ops)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("batch, seqlen, dim, dstate, forward", [(2, 1024, 512, 16, 16), (1, 3000, 200, 16, 32), (2, 700, 512, 24, 8)])
+def test_slots_of_a_row_in_pieces(dtype, batch, seqlen, dim, dstate, forward):
+    """Sequences that end inside a piece, at its last token and at the row's, each state from its own pieces."""
+    from causal_conv1d_b200 import ssm_scan
+
+    rows = [[96, 64, 1, 200, 31, -8, seqlen - 400], [seqlen]][:batch]
+    ops = to_dev(ref.case(151, batch, seqlen, dim, dstate, dtype=dtype, lengths=rows))
+    assert pieces(ops, False) == forward
+    _, h = ref.scan(**ref.wide(ops), dt_softplus=True)
+    cache = torch.full((9, dim, dstate), 7.0, device=DEV)
+    slots = torch.tensor([[4, 0, 8, 1, -1, 2], [3, 5, 5, 5, 5, 5]], device=DEV)[:batch]
+    ssm_scan(**ops, dt_softplus=True, ssm_state=cache, ssm_state_indices=slots)
+    ends = {4: (0, 95), 0: (0, 159), 8: (0, 160), 1: (0, 360), 2: (0, seqlen - 1), 3: (1, seqlen - 1)}
+    for slot, (b, t) in ends.items():
+        if b < batch:
+            ref.assert_near(cache[slot], h[b, t], seqlen, f"slot {slot}")
+            assert ((cache[slot].double() - h[b, t]).norm() / h[b, t].norm()) <= 1e-5  # check_norms
+    for slot in (5, 6, 7, *([3] if batch == 1 else [])):
+        assert (cache[slot] == 7).all()
+
+
+@pytest.mark.parametrize("dtype, state_dtype", [(BF16, F32), (F16, F16), (F32, F32), (BF16, BF16)])
+@pytest.mark.parametrize("batch, dim, dstate, groups", [
+    (77, 2030, 16, 2),   # two groups of rows a CTA, the last one of 5 rows, 14 channels in the last CTA of a row
+    (45, 1604, 32, 1),
+    (29, 1210, 64, 0),
+    (9, 100, 16, 0),     # one group a CTA
+    (9, 52, 32, 2),
+    (5, 20, 64, 1),
+])
+def test_decode_batches(dtype, state_dtype, batch, dim, dstate, groups):
+    """The one-token kernel with both counts of rows a CTA, rows and channels that fill no CTA, slots in any order."""
+    from causal_conv1d_b200 import ssm_scan, ssm_update
+
+    ops = to_dev(ref.case(157 + batch, batch, 1, dim, dstate, groups, dtype))
+    g = torch.Generator(device=DEV).manual_seed(batch)
+    state0 = torch.randn(batch + 3, dim, dstate, generator=g, device=DEV).to(state_dtype)
+    slots = torch.randperm(batch + 3, generator=g, device=DEV)[:batch]
+    skipped = torch.arange(batch, device=DEV) % 11 == 3
+    state = state0.clone()
+    out = ssm_update(ssm_state=state, dt_softplus=True, ssm_state_indices=torch.where(skipped, -1, slots), **token_ops(ops, 0))
+    full = dict(ops, initial_states=state0[slots].float())
+    wout, wh = ref.scan(**ref.wide(full), dt_softplus=True)
+    live = ~skipped
+    ref.assert_near(out[live], wout[live, 0], 1, "out")
+    ref.assert_near(state[slots[live]], wh[live, 0], 1, "state")
+    untouched = torch.ones(batch + 3, device=DEV, dtype=torch.bool)
+    untouched[slots[live]] = False
+    assert torch.equal(state[untouched], state0[untouched])
+    same, fin = ssm_scan(**full, dt_softplus=True, return_final_states=True)
+    assert torch.equal(out[live], same[live, 0])
+    if state_dtype == F32:
+        assert torch.equal(state[slots[live]], fin[live])
+
+
+def test_decode_after_a_prompt_in_pieces():
+    """A prompt cut in pieces, whose states come through the decay of a summed step, continued token by token:
+    within the tolerance of the 64-bit form over the whole sequence, which a scan of it keeps too."""
+    from causal_conv1d_b200 import ssm_scan, ssm_update
+
+    ops = to_dev(ref.case(163, 1, 520, 512, 16, dtype=BF16))
+    prompt = {k: v[:, :512] if k in ("x", "dt", "B", "C", "z") else v for k, v in ops.items()}
+    assert pieces(prompt, False) > 1
+    wout, wh = ref.scan(**ref.wide(ops), dt_softplus=True)
+    out, state = ssm_scan(**prompt, dt_softplus=True, return_final_states=True)
+    steps = [ssm_update(ssm_state=state, dt_softplus=True, **token_ops(ops, t)) for t in range(512, 520)]
+    ref.assert_near(torch.cat([out, torch.stack(steps, 1)], 1), wout, 520, "out")
+    ref.assert_near(state, wh[:, -1], 520, "state")
+    assert ((state.double() - wh[:, -1]).norm() / wh[:, -1].norm()) <= 1e-5  # check_norms
