@@ -11,7 +11,8 @@ The reference has the convolution alone; its README names the layer that calls i
 (causal-conv1d-triton README.md:3-4). Layouts, names and conventions are the convolution's:
 (batch, seqlen, dim) with channel stride 1 and any other strides, `seq_idx` for packed rows, states
 in and out, `*_update` with slot indices for decoding. fp32/fp16/bf16 inputs; all arithmetic, h and
-every sum are fp32. The kernels (csrc/cc1d_ssm_*.cu, csrc/cc1d_slot_maps.cu) are behind the C ABI of
+every sum are fp32. Integer tensors of other types are converted to int32, which their values have to
+fit. The kernels (csrc/cc1d_ssm_*.cu, csrc/cc1d_slot_maps.cu) are behind the C ABI of
 include/causal_conv1d_b200.h and run on torch's current stream. The argument checks and the autograd
 Function are C++ (csrc/cc1d_torch_ssm.cpp): AssertionError for shapes and devices, TypeError for
 element types, NotImplementedError for forward-mode derivatives (tensors with a tangent), CausalConv1dError

@@ -8,8 +8,9 @@
 // in flight together, A is read once, and the element-wise work (step size, gate) is shared out, each
 // of four lanes doing one row for all the channel's lanes. The sums over states go across lanes with
 // lane_sums, which leaves each row's on the lane that finishes it. Step, decay and state update are
-// the forward's operations in the forward's order, so that decoding continues a prompt with the
-// forward's bits.
+// the forward's operations in the forward's order: against an fp32 state, tokens give the bits of a forward
+// over them that runs in one piece. (Between pieces a forward carries states by one decay of the summed
+// steps, and a 16-bit state is rounded at every call.)
 #include <type_traits>
 
 #include "cc1d_ssm_device.cuh"
@@ -36,11 +37,11 @@ __device__ __forceinline__ void ld_any4(const void* base, int64_t i, int dtype, 
 // One token of every row, dstate 16, 32 or 64, all of it in aligned vectors: what a decode step is. A CTA
 // takes G groups of kRows rows of its channels and has all their states on the way at once, as
 // asynchronous copies of each thread's own pieces (16 KB a CTA at G = 2, eight CTAs an SM: with 256 threads
-// and four, 128 rows of 2048 channels take 9.2 us instead of 8.5, and 256 x 4352 0.5 us more). 256 rows of
-// 4352 channels, fp32 states, 151 MB: 31.6 us between other calls, 28.5 in a row of such steps (5.3 TB/s,
-// 0.81 of the measured copy bandwidth); against 32.5 before, 33.8 us with three groups, 35.4 with four (80 registers, three
-// quarters of the threads), 41 with the loads of a group in registers. Issue slots are 69% taken (124 instructions a
-// warp and row); addresses of one 32-bit product and B and C a group ahead are no faster.
+// and four, 128 rows of 2048 channels take 9.2 us instead of 8.5). 256 rows of 4352 channels, fp32 states, 151 MB:
+// 30.8 us between other calls, 28.5 in a row of such steps (5.3 TB/s, 0.81 of the measured copy
+// bandwidth); 33.8 us with three groups, 35.4 with four (80 registers, three quarters of the threads), 41 with the
+// loads of a group in registers. Issue slots are 69% taken (124 instructions a warp and row); addresses of one
+// 32-bit product and B and C a group ahead are no faster.
 template <typename T, typename ST, int NL, int G>
 __global__ void __launch_bounds__(kStep, 1024 / kStep) cc1d_ssm_step_kernel(const __grid_constant__ SsmUpdateParams p) {
   constexpr int BYTES = 4 * static_cast<int>(sizeof(ST));
@@ -141,9 +142,9 @@ __global__ void __launch_bounds__(kStep, 1024 / kStep) cc1d_ssm_step_kernel(cons
 
 // Any number of tokens, states and alignment, four rows a CTA. VEC: a lane's 4 states are one aligned
 // vector, and so are its B and C. 256 rows of 4352 channels, 16 states, inputs partly in L2: 78 us for 4
-// tokens (113 with a token's operands loaded where they are used and addressed by products), 131 us for
-// 8 (202): what bounds it is the issue and latency of a token's work at 16 warps an SM (125 registers).
-// Three CTAs an SM spill, and are slower but for the longest calls (77 and 124; 21 against 19 at 64 rows).
+// tokens, 131 us for 8; with a token's operands loaded where they are used and addressed by products 113 and 202.
+// What bounds it is the issue and latency of a token's work at 16 warps an SM (125 registers). Three CTAs an SM
+// spill, and are slower but for the longest calls (77 and 124; 21 against 19 at 64 rows).
 template <typename T, typename ST, int NL, bool VEC>
 __global__ void __launch_bounds__(256, 2) cc1d_ssm_update_kernel(const __grid_constant__ SsmUpdateParams p) {
   const int nl = threadIdx.x % NL, n0 = 4 * nl;
@@ -277,6 +278,9 @@ cudaError_t launch_step(SsmUpdateParams p, cudaStream_t s) {
 template <typename T, typename ST, int NL>
 cudaError_t launch(const SsmUpdateParams& p, cudaStream_t s) {
   const bool vec = p.dstate % 4 == 0 && reinterpret_cast<uintptr_t>(p.state) % (4 * sizeof(ST)) == 0 && p.Bm.vec && p.Cm.vec;
+  // The one-token kernel has no lane without states, which it would have to mask in its copies, stores and loads
+  // of A, B and C: 4, 8, 12 or 20 states take the general kernel, also where they are aligned (256 rows of 4352
+  // channels, fp32 states: 4 states 39 us, 8 42, 12 45, against 31 for 16).
   if (vec && p.seqlen == 1 && p.dstate == 4 * NL) {
     // Two groups a CTA where that leaves 512 threads for every SM, one for small batches. States out of the
     // caches, one group against two: 1 x 512 channels 2.1 and 2.7 us, 48 x 2048 4.1 and 4.4, 64 x 2048 5.2 and 5.8
