@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 2) cc1d_ssm_scan_kernel(const __grid
 
 // What each piece receives, from the pieces' own results: forward, the state that the pieces before
 // leave it; backward, the gradient that the pieces after pass to it. One thread per state; its loads
-// are independent of the chain.
+// are independent of the chain, which tests for 0 times infinity only where it gave a NaN, as piece_in does.
 __global__ void __launch_bounds__(128) cc1d_ssm_join_kernel(const float* __restrict__ own, const float* __restrict__ decay,
                                                             float* __restrict__ in, int segs, int64_t row, int64_t n,
                                                             bool backward) {
@@ -361,12 +361,16 @@ __global__ void __launch_bounds__(128) cc1d_ssm_join_kernel(const float* __restr
   const int64_t step = backward ? -row : row, first = (i / row) * segs * row + i % row;
   const int64_t at = backward ? first + (segs - 1) * row : first;
   float carry = own[at];
-#pragma unroll 8
-  for (int s = 1; s < segs - 1; ++s) {
-    const float o = own[at + s * step], d = decay[at + s * step];
-    in[at + s * step] = carry;
-    carry = pass_piece(d, carry, o);
+  constexpr int N = 8;
+  int s = 1;
+  for (; s + N <= segs - 1; s += N) {
+    float o[N], d[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) o[k] = own[at + (s + k) * step], d[k] = decay[at + (s + k) * step];
+#pragma unroll
+    for (int k = 0; k < N; ++k) in[at + (s + k) * step] = carry, carry = pass_piece(d[k], carry, o[k]);
   }
+  for (; s < segs - 1; ++s) in[at + s * step] = carry, carry = pass_piece(decay[at + s * step], carry, own[at + s * step]);
   in[at + (segs - 1) * step] = carry;  // the last piece's own result is not needed and was not computed
 }
 
