@@ -6,6 +6,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -110,10 +111,16 @@ int occupancy(const KernelInfo& k, int max_smem, int dev, int* occ) {
 // For the entry points in other files.
 int record_cuda_error(cudaError_t e) { return cuda_fail(e); }
 int device_sms(int* sms) {
-  DeviceInfo di;
+  // Kept apart from DeviceInfo: a decode step asks at every call, without the lock and the copy of that.
+  static std::atomic<int> known[kMaxDevices];
   int dev = 0;
-  CC1D_TRY(device_info(&di, &dev));
-  *sms = di.sms;
+  CC1D_TRY_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return CC1D_ERR_INVALID;
+  *sms = known[dev].load(std::memory_order_relaxed);
+  if (*sms == 0) {
+    CC1D_TRY_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    known[dev].store(*sms, std::memory_order_relaxed);
+  }
   return CC1D_OK;
 }
 

@@ -10,6 +10,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/extension.h>
 
 #include <initializer_list>
@@ -119,8 +120,10 @@ void check_operands(const at::Tensor& x, const at::Tensor& dt, const at::Tensor&
 }
 
 // Forward-mode derivatives: the kernels have none, and tensors that carry a tangent (torch.autograd.forward_ad)
-// would come out without one, which reads as a derivative of zero.
+// would come out without one, which reads as a derivative of zero. Tensors have tangents only inside a
+// forward-mode level; torch allows one, of index 0, and asking for it costs less than asking every operand.
 void refuse_tangents(std::initializer_list<const at::Tensor*> given, std::initializer_list<const Opt*> optional) {
+  if (torch::autograd::ForwardADLevel::try_get_by_idx(0) == nullptr) return;
   auto check = [](const at::Tensor& t) {
     if (t._fw_grad(0).defined()) raise(PyExc_NotImplementedError, "the state-space operators have no forward-mode derivatives");
   };
