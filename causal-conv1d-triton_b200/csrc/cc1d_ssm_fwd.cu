@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 2) cc1d_ssm_scan_kernel(const __grid
 // What each piece receives, from the pieces' own results: forward, the state that the pieces before
 // leave it; backward, the gradient that the pieces after pass to it. One thread per state; its loads
 // are independent of the chain, and those of eight pieces are gathered before pass_piece's branches, which
-// would keep them from being issued early (85.5 us instead of 84.0 for 21230 tokens x 171 channels).
+// would keep them from being issued early (83.5 us instead of 82.0 for 21230 tokens x 171 channels).
 __global__ void __launch_bounds__(128) cc1d_ssm_join_kernel(const float* __restrict__ own, const float* __restrict__ decay,
                                                             float* __restrict__ in, int segs, int64_t row, int64_t n,
                                                             bool backward) {
